@@ -14,10 +14,14 @@ from .session import MatrelSession
 from .blocks.matrix import BlockMatrix
 from .blocks import schemes
 from .exec.runtime import get_runtime, init_runtime
+from .ops.fp8 import Fp8Blocks, fp8_matmul, quantize_fp8
+from .ops.grouped import grouped_matmul, grouped_matmul_grads
 
 __version__ = "0.1.0"
 
 __all__ = [
     "MatrelConfig", "get_config", "set_config", "Matrix", "MatrelSession",
     "BlockMatrix", "schemes", "get_runtime", "init_runtime",
+    "Fp8Blocks", "fp8_matmul", "quantize_fp8",
+    "grouped_matmul", "grouped_matmul_grads",
 ]

@@ -581,6 +581,8 @@ std::vector<torch::Tensor> transpose_batch(std::vector<torch::Tensor> ts) {
 
 }  // namespace
 
+void bind_grouped(pybind11::module& m);  // ext_grouped.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "matrel_amd hand-written CDNA4 (gfx950) kernels";
   m.def("gemm_bt_acc", &gemm_bt_acc,
@@ -645,4 +647,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "C(f32) += A6 @ Bt6^T (MX-fp6 scaled MFMA at the fp4 rate)");
   m.def("gemm_bt_mx8_acc", &gemm_bt_mx8_acc,
         "C(f32) += A8 @ Bt8^T (MX-fp8 scaled MFMA, ~2x bf16 rate)");
+  bind_grouped(m);
 }

@@ -1,0 +1,314 @@
+// Python bindings of the grouped products and of the 8-bit block conversion.
+// Host-side only: what the kernels assume of shapes, strides and alignment is
+// checked or chosen here.
+#include <torch/extension.h>
+#include <torch/csrc/autograd/variable.h>
+#include <c10/hip/HIPGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+
+#include <limits>
+#include <tuple>
+
+#include "grouped_args.h"
+
+extern "C" {
+void launch_grouped_bf16(const GroupedArgs*, int, int, int, int, hipStream_t);
+void launch_grouped_f16(const GroupedArgs*, int, int, int, int, hipStream_t);
+void launch_grouped_f32(const GroupedArgs*, int, int, int, int, hipStream_t);
+void launch_grouped_fp8(const GroupedArgs*, int, int, hipStream_t);
+void launch_grouped_join(const float*, void*, long, int, int, hipStream_t);
+void launch_fp8_quantize_row(const void*, int, long, long, long, void*,
+                             float*, int, hipStream_t);
+void launch_fp8_quantize_tile(const void*, int, long, long, long, long, long,
+                              void*, void*, float*, float*, int, hipStream_t);
+}
+
+namespace {
+
+using torch::Tensor;
+
+int type_of(at::ScalarType t) {
+  switch (t) {
+    case torch::kBFloat16: return GT_BF16;
+    case torch::kFloat16: return GT_F16;
+    case torch::kFloat32: return GT_F32;
+    case torch::kFloat8_e4m3fn: return GT_FP8;
+    default: TORCH_CHECK(false, "unsupported type ", t);
+  }
+}
+
+hipStream_t stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+void check_launch() {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, "HIP error: ", hipGetErrorString(e));
+}
+
+int dim32(int64_t n, const char* what) {
+  TORCH_CHECK(n >= 0 && n < (int64_t(1) << 31) - 512, what, " is too large");
+  return (int)n;
+}
+
+// Rows (or k) of `ld` elements that begin on 16 bytes.
+bool aligned(const Tensor& t, int64_t ld, int64_t count) {
+  const int64_t es = t.element_size();
+  return (uintptr_t)t.data_ptr() % 16 == 0 &&
+         (count <= 1 || ld * es % 16 == 0);
+}
+
+void set_offsets(GroupedArgs& p, const c10::optional<Tensor>& offs,
+                 const Tensor& a, int64_t groups) {
+  if (!offs.has_value()) {
+    TORCH_CHECK(groups == 1, "several groups need offsets");
+    return;
+  }
+  TORCH_CHECK(offs->device() == a.device() && offs->dim() == 1 &&
+                  offs->is_contiguous() && offs->numel() == groups + 1 &&
+                  (offs->scalar_type() == torch::kInt32 ||
+                   offs->scalar_type() == torch::kInt64),
+              "offsets must be groups + 1 integers on the operands' device");
+  p.offs = offs->data_ptr();
+  p.off64 = offs->scalar_type() == torch::kInt64;
+}
+
+// 2: 256 x 256, 1: 128 x 128, 0: 32 x 128
+int choose_tile(int64_t rows_each, int64_t M, int64_t N) {
+  if (rows_each > 128 && N > 128) return 2;
+  return rows_each > 32 ? 1 : 0;
+}
+
+void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
+                 hipStream_t s) {
+  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, s);
+  else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, fast, s);
+  else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, fast, s);
+  else launch_grouped_f32(&p, tile, bk, 0, fast, s);
+  check_launch();
+}
+
+// c[t, :] = a[t, :] @ b[group of t], zeros for rows of no group.
+// a [T, K], last dimension contiguous; b [E, K, N], k or n contiguous.
+Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
+                    at::ScalarType out) {
+  TORCH_CHECK(a.is_cuda() && b.device() == a.device(),
+              "operands must be on one GPU");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 3 && a.size(1) == b.size(1) &&
+              a.scalar_type() == b.scalar_type(), "operands do not match");
+  const c10::hip::HIPGuard guard(a.device().index());
+  const int64_t T = a.size(0), K = a.size(1), N = b.size(2), E = b.size(0);
+  GroupedArgs p = {};
+  p.T = dim32(T, "rows");
+  p.K = dim32(K, "inner size");
+  p.N = dim32(N, "columns");
+  p.E = dim32(E, "groups");
+  const int ty = type_of(a.scalar_type());
+  TORCH_CHECK(ty != GT_FP8);
+  set_offsets(p, offs, a, E);
+  Tensor c = torch::empty({T, N}, a.options().dtype(out));
+  if (c.numel() == 0) return c;
+  if (E == 0 || K == 0) return c.zero_();
+  TORCH_CHECK(K == 1 || a.stride(1) == 1, "rows of a must be contiguous");
+  const bool bk = K == 1 || b.stride(1) == 1;
+  TORCH_CHECK(bk || N == 1 || b.stride(2) == 1,
+              "b must be contiguous along one of its matrix dimensions");
+  const int64_t epc = 16 / a.element_size();
+  p.a = a.data_ptr();
+  p.b = b.data_ptr();
+  p.c = c.data_ptr();
+  p.lda = T > 1 ? a.stride(0) : 0;
+  p.ldb = bk ? (N > 1 ? b.stride(2) : 0) : b.stride(1);
+  p.gsb = E > 1 ? b.stride(0) : 0;
+  p.splits = 1;
+  p.out = type_of(out);
+  const bool fast = aligned(a, p.lda, T) &&
+                    aligned(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
+                    (bk || N % epc == 0);
+  const int tile = choose_tile(T / E, T, N);
+  launch_rows(p, ty, tile, bk, fast, stream_of(a));
+  return c;
+}
+
+// c[g] = a_g^T @ b_g over the rows of each group, zeros for an empty one.
+// a [T, M], b [T, N], last dimensions contiguous.
+Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
+                       int64_t E, at::ScalarType out) {
+  TORCH_CHECK(a.is_cuda() && b.device() == a.device(),
+              "operands must be on one GPU");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.size(0) == b.size(0) &&
+              a.scalar_type() == b.scalar_type(), "operands do not match");
+  const c10::hip::HIPGuard guard(a.device().index());
+  const int64_t T = a.size(0), M = a.size(1), N = b.size(1);
+  GroupedArgs p = {};
+  p.T = dim32(T, "rows");
+  p.M = dim32(M, "columns of a");
+  p.N = dim32(N, "columns of b");
+  p.K = p.T;
+  p.E = dim32(E, "groups");
+  const int ty = type_of(a.scalar_type());
+  TORCH_CHECK(ty != GT_FP8);
+  set_offsets(p, offs, a, E);
+  Tensor c = torch::empty({E, M, N}, a.options().dtype(out));
+  if (c.numel() == 0) return c;
+  if (T == 0) return c.zero_();
+  TORCH_CHECK((M == 1 || a.stride(1) == 1) && (N == 1 || b.stride(1) == 1),
+              "rows must be contiguous");
+  const int64_t epc = 16 / a.element_size();
+  p.a = a.data_ptr();
+  p.b = b.data_ptr();
+  p.c = c.data_ptr();
+  p.lda = T > 1 ? a.stride(0) : 0;
+  p.ldb = T > 1 ? b.stride(0) : 0;
+  p.splits = 1;
+  p.out = type_of(out);
+  const bool fast = aligned(a, p.lda, T) && aligned(b, p.ldb, T) &&
+                    M % epc == 0 && N % epc == 0;
+  const int tile = choose_tile(M, T, N);
+  const hipStream_t s = stream_of(a);
+  if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, fast, s);
+  else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, fast, s);
+  else launch_grouped_f32(&p, tile, 0, 1, fast, s);
+  check_launch();
+  return c;
+}
+
+// c = a @ bt[group]^T of e4m3 operands: a [T, K] with scales [kb][T], bt
+// [E, N, K] with scales [E][kb][nb]. With `into` (f32, contiguous), the
+// product is written there, or added where `accum` is set.
+Tensor grouped_rows_fp8(Tensor a, Tensor asc, Tensor bt, Tensor bsc,
+                        c10::optional<Tensor> offs, at::ScalarType out,
+                        c10::optional<Tensor> into, bool accum) {
+  TORCH_CHECK(a.is_cuda() && bt.device() == a.device() &&
+              asc.device() == a.device() && bsc.device() == a.device(),
+              "operands must be on one GPU");
+  TORCH_CHECK(a.dim() == 2 && bt.dim() == 3 && a.size(1) == bt.size(2) &&
+              a.scalar_type() == torch::kFloat8_e4m3fn &&
+              bt.scalar_type() == torch::kFloat8_e4m3fn &&
+              a.is_contiguous() && bt.is_contiguous(),
+              "operands do not match");
+  const c10::hip::HIPGuard guard(a.device().index());
+  const int64_t T = a.size(0), K = a.size(1), N = bt.size(1), E = bt.size(0);
+  const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
+  TORCH_CHECK(asc.scalar_type() == torch::kFloat32 && asc.is_contiguous() &&
+              asc.dim() == 2 && asc.size(0) == kb && asc.size(1) == T,
+              "scales of a must be float32 [ceil(K/128), rows]");
+  TORCH_CHECK(bsc.scalar_type() == torch::kFloat32 && bsc.is_contiguous() &&
+              bsc.dim() == 3 && bsc.size(0) == E && bsc.size(1) == kb &&
+              bsc.size(2) == nb,
+              "scales of bt must be float32 [groups, ceil(K/128), "
+              "ceil(N/128)]");
+  GroupedArgs p = {};
+  p.T = dim32(T, "rows");
+  p.K = dim32(K, "inner size");
+  p.N = dim32(N, "columns");
+  p.E = dim32(E, "groups");
+  set_offsets(p, offs, a, E);
+  Tensor c;
+  if (into.has_value()) {
+    c = *into;
+    TORCH_CHECK(c.scalar_type() == torch::kFloat32 && c.is_contiguous() &&
+                c.device() == a.device() && c.dim() == 2 && c.size(0) == T &&
+                c.size(1) == N, "the result must be float32 [rows, columns]");
+  } else {
+    c = torch::empty({T, N}, a.options().dtype(out));
+  }
+  if (c.numel() == 0) return c;
+  if (E == 0 || K == 0) return accum ? c : c.zero_();
+  p.a = a.data_ptr();
+  p.b = bt.data_ptr();
+  p.c = c.data_ptr();
+  p.asc = asc.data_ptr<float>();
+  p.bsc = bsc.data_ptr<float>();
+  p.lda = T > 1 ? K : 0;
+  p.ldb = N > 1 ? K : 0;
+  p.gsb = E > 1 ? N * K : 0;
+  p.splits = 1;
+  p.out = type_of(c.scalar_type());
+  p.accum = accum;
+  const bool fast = aligned(a, p.lda, T) && aligned(bt, p.ldb, N) &&
+                    aligned(bt, p.gsb, E);
+  launch_rows(p, GT_FP8, choose_tile(T / E, T, N), true, fast, stream_of(a));
+  return c;
+}
+
+// [R, C] -> (e4m3 [R, C], scales [ceil(C/128), R])
+std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2);
+  const c10::hip::HIPGuard guard(x.device().index());
+  const int64_t R = x.size(0), C = x.size(1);
+  TORCH_CHECK(C <= 1 || x.stride(1) == 1, "rows must be contiguous");
+  const int ty = type_of(x.scalar_type());
+  TORCH_CHECK(ty != GT_FP8);
+  Tensor q = torch::empty({R, C}, x.options().dtype(torch::kFloat8_e4m3fn));
+  Tensor s = torch::empty({(C + 127) / 128, R},
+                          x.options().dtype(torch::kFloat32));
+  if (q.numel() == 0) return {q, s};
+  TORCH_CHECK((C + 127) / 128 * ((R + 15) / 16) < (int64_t(1) << 31),
+              "matrix is too large");
+  const int64_t ld = R > 1 ? x.stride(0) : 0;
+  launch_fp8_quantize_row(x.data_ptr(), ty, ld, R, C, q.data_ptr(),
+                          s.data_ptr<float>(), aligned(x, ld, R),
+                          stream_of(x));
+  check_launch();
+  return {q, s};
+}
+
+// [E, R, C] -> (e4m3 [E, R, C], scales [E, ceil(C/128), ceil(R/128)]), and
+// with `both` the same for the transposed matrices.
+std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
+                                                             bool both) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 3);
+  const c10::hip::HIPGuard guard(x.device().index());
+  const int64_t E = x.size(0), R = x.size(1), C = x.size(2);
+  TORCH_CHECK(C <= 1 || x.stride(2) == 1, "rows must be contiguous");
+  const int ty = type_of(x.scalar_type());
+  TORCH_CHECK(ty != GT_FP8);
+  const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128;
+  const auto o8 = x.options().dtype(torch::kFloat8_e4m3fn);
+  const auto of = x.options().dtype(torch::kFloat32);
+  Tensor q = torch::empty({E, R, C}, o8), s = torch::empty({E, cb, rb}, of);
+  Tensor qt, st;
+  if (both) {
+    qt = torch::empty({E, C, R}, o8);
+    st = torch::empty({E, rb, cb}, of);
+  } else {
+    qt = torch::empty({0}, o8);
+    st = torch::empty({0}, of);
+  }
+  if (q.numel() == 0) return {q, s, qt, st};
+  TORCH_CHECK(rb * cb < (int64_t(1) << 31) && E < 65536,
+              "matrix is too large");
+  const int64_t ld = R > 1 ? x.stride(1) : 0, bld = E > 1 ? x.stride(0) : 0;
+  launch_fp8_quantize_tile(x.data_ptr(), ty, ld, bld, E, R, C, q.data_ptr(),
+                           both ? qt.data_ptr() : nullptr,
+                           s.data_ptr<float>(),
+                           both ? st.data_ptr<float>() : nullptr,
+                           aligned(x, ld, R) && aligned(x, bld, E),
+                           stream_of(x));
+  check_launch();
+  return {q, s, qt, st};
+}
+
+// Whether an autograd graph that still lives accumulates into this leaf.
+bool has_grad_accumulator(const Tensor& t) {
+  return t.requires_grad() && t.is_leaf() &&
+         torch::autograd::impl::try_get_grad_accumulator(t) != nullptr;
+}
+
+}  // namespace
+
+void bind_grouped(pybind11::module& m) {
+  m.def("grouped_rows", &grouped_rows,
+        "rows of each group times the group's matrix");
+  m.def("grouped_weights", &grouped_weights,
+        "each group's a^T @ b over its rows");
+  m.def("grouped_rows_fp8", &grouped_rows_fp8,
+        "grouped product of e4m3 operands with block scales");
+  m.def("fp8_quantize_row", &fp8_quantize_row,
+        "e4m3 with a scale for each 128 of a row");
+  m.def("fp8_quantize_tile", &fp8_quantize_tile,
+        "e4m3 with a scale for each 128 x 128 tile");
+  m.def("has_grad_accumulator", &has_grad_accumulator);
+}

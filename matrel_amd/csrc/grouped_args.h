@@ -1,0 +1,21 @@
+// What the host hands to the grouped products.
+#pragma once
+
+enum GroupedType { GT_BF16 = 0, GT_F16 = 1, GT_F32 = 2, GT_FP8 = 3 };
+
+struct GroupedArgs {
+  const void* a;      // rows: [T][K]; weights: [T][M]
+  const void* b;      // rows: [E] of (n, k); weights: [T][N]
+  void* c;            // rows: [T][N]; weights: [E][M][N]
+  float* part;        // f32 partial sums [splits][...], null if splits == 1
+  const void* offs;   // E + 1 offsets, null: one group of all rows
+  const float* asc;   // fp8: scales of a, [ceil(K/128)][T]
+  const float* bsc;   // fp8: scales of b, [E][ceil(K/128)][ceil(N/128)]
+  long lda, ldb;      // elements from one row (or one k) to the next
+  long gsb;           // rows: elements from one group's b to the next
+  int T, M, N, K, E;
+  int off64;          // offsets are 64-bit
+  int splits;
+  int out;            // GroupedType of c
+  int accum;          // add to c (f32, one split)
+};

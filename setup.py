@@ -28,6 +28,12 @@ sources = [
     os.path.join(CSRC, "gemm_mx4.hip"),
     os.path.join(CSRC, "gemm_mx6.hip"),
     os.path.join(CSRC, "mxconvert.hip"),
+    os.path.join(CSRC, "ext_grouped.cpp"),
+    os.path.join(CSRC, "fp8.hip"),
+    os.path.join(CSRC, "grouped_bf16.hip"),
+    os.path.join(CSRC, "grouped_f16.hip"),
+    os.path.join(CSRC, "grouped_f32.hip"),
+    os.path.join(CSRC, "grouped_fp8.hip"),
 ]
 
 setup(

@@ -1,0 +1,475 @@
+"""Grouped products and 8-bit block products against plain float64 forms.
+
+Tolerances: a sum of K float32 products, in any order and with at most one
+step lost at each addition, is within (K + 8) * 2^-23 * sum |a b| of the exact
+one (8: the operations on scales); rounding the sum to the result's type adds
+half a step, eps / 2 relative to the value."""
+
+import math
+
+import pytest
+import torch
+
+import matrel_amd as ma
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+UNIT = 2.0 ** -23
+
+
+def randn(*shape, seed, dtype=torch.float32, device="cpu", scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(device)
+
+
+def offsets_of(sizes, device, dtype=torch.int32, head=0):
+    v = [head]
+    for s in sizes:
+        v.append(v[-1] + s)
+    return torch.tensor(v, dtype=dtype, device=device)
+
+
+def assert_near(got, exact, size, depth):
+    """got against the float64 result; size: the sums of |products|."""
+    exact, size = exact.cpu(), size.cpu()
+    err = (depth + 8) * UNIT * size
+    half = torch.finfo(got.dtype).eps / 2
+    tol = err + half * (exact.abs() + err)
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half a step of its subnormal values
+    off = (got.detach().cpu().double() - exact).abs()
+    assert torch.isfinite(off).all()
+    bad = off > tol
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} off, worst "
+                           f"{(off / tol.clamp(min=1e-300)).max():.3g} x tol "
+                           f"at {bad.nonzero()[0].tolist()}")
+
+
+def plain_rows(a, b, off):
+    """(result, sums of |products|) in float64; rows of no group zero."""
+    a, b, off = a.detach().cpu().double(), b.detach().cpu().double(), \
+        off.tolist()
+    y = torch.zeros(a.shape[0], b.shape[2], dtype=torch.float64)
+    s = torch.zeros_like(y)
+    for g, (lo, hi) in enumerate(zip(off, off[1:])):
+        y[lo:hi] = a[lo:hi] @ b[g]
+        s[lo:hi] = a[lo:hi].abs() @ b[g].abs()
+    return y, s
+
+
+def plain_weights(a, b, off):
+    a, b, off = a.detach().cpu().double(), b.detach().cpu().double(), \
+        off.tolist()
+    parts = [(a[lo:hi], b[lo:hi]) for lo, hi in zip(off, off[1:])]
+    return (torch.stack([x.t() @ y for x, y in parts]),
+            torch.stack([x.abs().t() @ y.abs() for x, y in parts]))
+
+
+# sizes of groups, k, n: one row, empty groups, tiles that end early, sizes
+# on and around the tiles' edges, rows that do not begin on 16 bytes
+SHAPES = [
+    ([1], 1, 1),
+    ([1], 64, 16),
+    ([0, 0, 3, 0], 40, 24),
+    ([5, 0, 1, 130, 31], 72, 136),
+    ([33, 64, 32], 128, 128),
+    ([129, 1, 255, 256, 257], 192, 264),
+    ([300, 290], 264, 520),
+    ([7, 200, 0, 61], 77, 111),
+    ([17, 3], 1000, 9),
+    ([0, 0], 16, 16),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("sizes,k,n", SHAPES)
+def test_grouped_matmul(sizes, k, n, layout, dtype, device):
+    off = offsets_of(sizes, device)
+    t = sum(sizes)
+    a = randn(t, k, seed=1, dtype=dtype, device=device)
+    if layout == "kn":
+        b = randn(len(sizes), k, n, seed=2, dtype=dtype, device=device)
+    else:
+        b = randn(len(sizes), n, k, seed=2, dtype=dtype,
+                  device=device).transpose(1, 2)
+    a.requires_grad_()
+    b.requires_grad_()
+    y = ma.grouped_matmul(a, b, off)
+    assert y.shape == (t, n) and y.dtype == dtype
+    assert_near(y, *plain_rows(a, b, off), k)
+    gy = randn(t, n, seed=3, dtype=dtype, device=device)
+    da, db = torch.autograd.grad(y, (a, b), gy)
+    assert da.dtype == db.dtype == dtype
+    assert_near(da, *plain_rows(gy, b.transpose(1, 2), off), n)
+    assert_near(db, *plain_weights(a, gy, off), max(sizes))
+    da2, db2 = ma.grouped_matmul_grads(gy, a, b, off)
+    assert torch.equal(da, da2) and torch.equal(db, db2)
+    assert not da2.requires_grad and not db2.requires_grad
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_many_groups(device):
+    """More groups than lanes of a wave, most of them empty."""
+    sizes = [(i * 7) % 5 if i % 3 == 0 else 0 for i in range(200)]
+    for dtype in (torch.int32, torch.int64):
+        off = offsets_of(sizes, device, dtype)
+        a = randn(sum(sizes), 64, seed=4, dtype=torch.bfloat16,
+                  device=device)
+        b = randn(200, 64, 40, seed=5, dtype=torch.bfloat16, device=device)
+        y = ma.grouped_matmul(a, b, off)
+        assert_near(y, *plain_rows(a, b, off), 64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_rows_of_no_group(device):
+    """Rows before the first and behind the last offset: zeros, zero
+    gradients, and nothing of theirs (NaN here) reaches a neighbour."""
+    off = offsets_of([20, 0, 45], device, head=3)
+    a = randn(80, 72, seed=6, dtype=torch.bfloat16, device=device)
+    a[:3], a[68:] = float("nan"), float("inf")
+    b = randn(3, 72, 40, seed=7, dtype=torch.bfloat16, device=device)
+    a.requires_grad_()
+    b.requires_grad_()
+    y = ma.grouped_matmul(a, b, off)
+    clean = a.detach().clone()
+    clean[:3], clean[68:] = 0, 0
+    assert_near(y, *plain_rows(clean, b, off), 72)
+    assert (y[:3] == 0).all() and (y[68:] == 0).all()
+    gy = randn(80, 40, seed=8, dtype=torch.bfloat16, device=device)
+    gy[:3], gy[68:] = float("inf"), float("nan")
+    da, db = torch.autograd.grad(y, (a, b), gy)
+    assert (da[:3] == 0).all() and (da[68:] == 0).all()
+    gy[:3], gy[68:] = 0, 0
+    assert_near(db, *plain_weights(clean, gy, off), 45)
+    assert (db[1] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_nonfinite_stays_in_its_group(device):
+    off = offsets_of([10, 22], device)
+    a = randn(32, 64, seed=9, dtype=torch.float16, device=device)
+    a[4, 5] = float("nan")
+    b = randn(2, 64, 32, seed=10, dtype=torch.float16, device=device)
+    b[0, 0, 0] = float("inf")
+    y = ma.grouped_matmul(a, b, off)
+    assert torch.isnan(y[4]).all()
+    assert not torch.isfinite(y[:10, 0]).any()
+    assert torch.isfinite(y[10:]).all()
+    db = ma.grouped_matmul_grads(torch.ones_like(y), a, b, off)[1]
+    assert torch.isnan(db[0, 5]).all() and torch.isfinite(db[1]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_strides(device):
+    """Row strides, offset views, expanded operands, other orders."""
+    off = offsets_of([9, 40, 15], device)
+    big = randn(64, 200, seed=11, dtype=torch.bfloat16, device=device)
+    w = randn(3, 96, 80, seed=12, dtype=torch.bfloat16, device=device)
+    for a in (big[:, :96], big[:, 8:104], big[:, 3:99],
+              randn(96, 64, seed=13, dtype=torch.bfloat16,
+                    device=device).t()):
+        y = ma.grouped_matmul(a, w, off)
+        assert_near(y, *plain_rows(a, w, off), 96)
+    a = big[:, :96]
+    wide = randn(3, 96, 90, seed=14, dtype=torch.bfloat16, device=device)
+    flat = randn(3 * 97 * 83, seed=15, dtype=torch.bfloat16, device=device)
+    for b in (wide[:, :, :80], wide[:, :, 5:85], w[:1].expand(3, 96, 80),
+              flat.as_strided((3, 96, 80), (97 * 83, 83, 1)),
+              flat.as_strided((3, 96, 80), (97 * 83, 1, 97)),
+              randn(96, 80, 3, seed=16, dtype=torch.bfloat16,
+                    device=device).permute(2, 0, 1)):
+        y = ma.grouped_matmul(a, b, off)
+        assert_near(y, *plain_rows(a, b, off), 96)
+    # a broadcast matrix sums the gradients of all groups
+    shared = w[0].clone().requires_grad_()
+    y = ma.grouped_matmul(a, shared.expand(3, 96, 80), off)
+    y.float().sum().backward()
+    one = torch.ones(64, 80)
+    parts, size = plain_weights(a, one, off)
+    exact, size = parts.sum(0), size.sum(0)
+    # each group's gradient is rounded once, their sum at most twice more
+    tol = size * (64 + 8) * UNIT + 2.0 ** -8 * 3.1 * parts.abs().sum(0)
+    assert ((shared.grad.cpu().double() - exact).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_out_dtype(device):
+    off = offsets_of([30, 70], device)
+    a = randn(100, 136, seed=17, dtype=torch.bfloat16, device=device)
+    b = randn(2, 136, 72, seed=18, dtype=torch.bfloat16, device=device)
+    y = ma.grouped_matmul(a, b, off, out_dtype=torch.float32)
+    assert y.dtype == torch.float32
+    assert_near(y, *plain_rows(a, b, off), 136)
+    a.requires_grad_()
+    y = ma.grouped_matmul(a, b, off, out_dtype=torch.float32)
+    da, = torch.autograd.grad(y.sum(), a)
+    assert da.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_empty(device):
+    f = dict(dtype=torch.bfloat16, device=device)
+    off = offsets_of([0, 0], device)
+    y = ma.grouped_matmul(torch.zeros(0, 8, **f), torch.zeros(2, 8, 4, **f),
+                          off)
+    assert y.shape == (0, 4)
+    a, b = torch.ones(5, 0, **f), torch.ones(2, 0, 4, **f)
+    y = ma.grouped_matmul(a, b, offsets_of([2, 3], device))
+    assert y.shape == (5, 4) and (y == 0).all()
+    y = ma.grouped_matmul(torch.ones(5, 8, **f), torch.ones(0, 8, 4, **f),
+                          torch.zeros(1, dtype=torch.int32, device=device))
+    assert y.shape == (5, 4) and (y == 0).all()
+    a = torch.ones(0, 8, **f).requires_grad_()
+    b = torch.ones(2, 8, 4, **f).requires_grad_()
+    y = ma.grouped_matmul(a, b, off)
+    da, db = torch.autograd.grad(y.sum(), (a, b))
+    assert da.shape == (0, 8) and (db == 0).all()
+
+
+def test_grouped_gradient_by_differences():
+    """The CPU form in float32 against central differences."""
+    off = offsets_of([3, 0, 4], "cpu")
+    a = randn(8, 6, seed=19).requires_grad_()
+    b = randn(3, 6, 5, seed=20).requires_grad_()
+    gy = randn(8, 5, seed=21)
+    da, db = torch.autograd.grad(ma.grouped_matmul(a, b, off), (a, b), gy)
+
+    def loss(x, w):
+        return float((plain_rows(x, w, off)[0] * gy.double()).sum())
+
+    for t, d, f in ((a, da, lambda v: loss(v, b)),
+                    (b, db, lambda v: loss(a, v))):
+        for i in range(0, t.numel(), 7):
+            step = torch.zeros(t.numel(), dtype=torch.float64)
+            step[i] = 1e-3
+            step = step.reshape(t.shape)
+            x = t.detach().double()
+            # bilinear: the central difference is exact but for rounding
+            diff = (f(x + step) - f(x - step)) / 2e-3
+            assert abs(diff - float(d.reshape(-1)[i])) < 1e-4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_grouped_refusals(device):
+    a = torch.zeros(8, 16, dtype=torch.bfloat16, device=device)
+    b = torch.zeros(2, 16, 4, dtype=torch.bfloat16, device=device)
+    off = offsets_of([3, 5], device)
+    bad = [
+        (a[0], b, off), (a, b[0], off), (a[:, :8], b, off),
+        (a, b, off[:2]), (a, b, off.reshape(1, 3)),
+        (a.float(), b, off), (a.double(), b.double(), off),
+        (a, b, off.float()), (a, b, [0, 3, 8]), ([1.0], b, off),
+        (a.to_sparse_csr(), b, off),
+    ]
+    if device == "cpu":
+        bad += [(a, b, torch.tensor([0, 5, 3])),
+                (a, b, torch.tensor([0, 3, 9])),
+                (a, b, torch.tensor([-1, 3, 8]))]
+    else:
+        bad += [(a, b, off.cpu()), (a, b.cpu(), off)]
+    for args in bad:
+        with pytest.raises((ValueError, TypeError)):
+            ma.grouped_matmul(*args)
+    with pytest.raises(TypeError):
+        ma.grouped_matmul(a, b, off, out_dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ma.grouped_matmul_grads(torch.zeros(8, 5, device=device), a, b, off)
+    a.requires_grad_()
+    y = ma.grouped_matmul(a, b, off)
+    g, = torch.autograd.grad(y.sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_grouped_bad_offsets_stay_inside():
+    """On a GPU the values are not looked at: offsets out of range or out of
+    order make wrong results but address nothing outside."""
+    a = randn(40, 64, seed=22, dtype=torch.bfloat16, device="cuda")
+    b = randn(3, 64, 32, seed=23, dtype=torch.bfloat16, device="cuda")
+    for v in ([0, 50, 100, 1 << 30], [-5, 10, 20, 40], [0, 30, 10, 40]):
+        off = torch.tensor(v, dtype=torch.int32, device="cuda")
+        y = ma.grouped_matmul(a, b, off)
+        _, db = ma.grouped_matmul_grads(y, a, b, off)
+        assert y.shape == (40, 32) and db.shape == b.shape
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------- 8-bit blocks ------
+
+def plain_quantize(x, kind):
+    """(values of the payload, scales [.., column blocks, row blocks]) from
+    the definition, the float32 steps in float32, the rest in float64."""
+    r, c = x.shape[-2:]
+    h = 1 if kind == "row" else 128
+    rb, cb = -(-r // h), -(-c // 128)
+    q = torch.zeros(x.shape, dtype=torch.float64)
+    s = torch.zeros(*x.shape[:-2], cb, rb)
+    most = torch.tensor(448.0)
+    for i in range(rb):
+        for j in range(cb):
+            b = x[..., i * h:(i + 1) * h, j * 128:(j + 1) * 128].float()
+            top = b.abs().flatten(-2).amax(-1)
+            top = torch.maximum(top, torch.full_like(top, 2.0 ** -100))
+            s[..., j, i] = top / most.expand_as(top)
+            v = (b * (most / top)[..., None, None]).double()
+            e = torch.frexp(v.abs())[1].clamp(min=-5) - 4
+            step = torch.pow(torch.tensor(2.0, dtype=torch.float64), e)
+            v = torch.round(v / step) * step
+            q[..., i * h:(i + 1) * h, j * 128:(j + 1) * 128] = v
+    return q, s
+
+
+def values_of(q):
+    """What blocks stand for, in float64."""
+    s = q.scale.cpu().double().transpose(-1, -2)
+    s = s.repeat_interleave(128, -1)[..., :q.shape[-1]]
+    if q.kind == "tile":
+        s = s.repeat_interleave(128, -2)[..., :q.shape[-2], :]
+    return q.data.cpu().float().double() * s
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["row", "tile"])
+@pytest.mark.parametrize("shape", [
+    (1, 1), (1, 128), (1, 1000), (16, 128), (17, 136), (130, 260),
+    (3, 5, 7), (2, 129, 384), (300, 64)])
+def test_quantize(shape, kind, dtype, device):
+    x = randn(*shape, seed=30, dtype=dtype, device=device, scale=3.0)
+    r = ma.quantize_fp8(x, kind)
+    q, s = plain_quantize(x.cpu(), kind)
+    assert r.data.dtype == torch.float8_e4m3fn and r.shape == x.shape
+    assert torch.equal(r.scale.cpu(), s)
+    assert torch.equal(r.data.cpu().float().double(), q)
+    assert torch.equal(r.dequantize().cpu(),
+                       values_of(r).to(torch.float32))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["row", "tile"])
+def test_quantize_special_values(kind, device):
+    x = torch.zeros(256, 512, device=device)
+    x[0, 0] = 1e-38             # its block stands for zeros
+    x[0, 128:256] = 3e38
+    x[0, 300] = float("nan")
+    x[0, 400] = float("-inf")
+    x[0, 511] = 5.0
+    x[200, 1] = 2.0 ** -100
+    r = ma.quantize_fp8(x, kind)
+    v = r.dequantize().cpu()
+    assert torch.equal(r.scale.cpu(), ma.quantize_fp8(x.cpu(), kind).scale) \
+        or torch.isnan(r.scale).any()
+    assert v[0, 0].abs() <= 2.0 ** -108
+    assert torch.allclose(v[0, 128:256], x[0, 128:256].cpu(), rtol=2 ** -4)
+    assert torch.isnan(v[0, 256:384]).all()
+    assert torch.isnan(v[0, 384:512]).all()
+    assert v[200, 1] == pytest.approx(2.0 ** -100, rel=2 ** -20)
+    if kind == "row":
+        assert (v[1:200] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_quantize_strides(device):
+    big = randn(90, 300, seed=31, dtype=torch.bfloat16, device=device)
+    for x in (big[:, :200], big[:, 8:208], big[:, 3:203], big[::2, :200],
+              big.t(), big[:1].expand(40, 300)):
+        for kind in ("row", "tile"):
+            r = ma.quantize_fp8(x, kind)
+            q, s = plain_quantize(x.cpu(), kind)
+            assert torch.equal(r.scale.cpu(), s)
+            assert torch.equal(r.data.cpu().float().double(), q)
+    assert ma.quantize_fp8(big[:0]).scale.shape == (3, 0)
+    assert ma.quantize_fp8(big[:, :0], "tile").scale.shape == (0, 1)
+
+
+def plain_fp8(a, bt, off, dtype):
+    """float64 product of what the blocks stand for."""
+    return plain_rows(values_of(a), values_of(bt).transpose(-1, -2), off)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,k,n", [
+    ([1], 1, 1), ([1], 128, 16), ([1], 4096, 200), ([40, 0, 3], 136, 24),
+    ([5, 0, 1, 130, 31], 256, 136), ([129, 257], 384, 264),
+    ([300, 290], 1000, 520), ([7, 61], 77, 111), ([3], 0, 5)])
+def test_fp8_matmul(sizes, k, n, dtype, device):
+    off = offsets_of(sizes, device)
+    a = randn(sum(sizes), k, seed=32, dtype=dtype, device=device)
+    w = randn(len(sizes), n, k, seed=33, dtype=dtype, device=device)
+    qa, qw = ma.quantize_fp8(a), ma.quantize_fp8(w, "tile")
+    want = plain_fp8(qa, qw, off, dtype)
+    y = ma.fp8_matmul(a, qw, off)
+    assert y.dtype == dtype
+    assert_near(y, *want, k + 128)
+    assert torch.equal(y, ma.fp8_matmul(a, w, off))
+    y = ma.fp8_matmul(qa, qw, off)
+    assert y.dtype == torch.bfloat16
+    assert_near(y, *want, k + 128)
+    y = ma.fp8_matmul(qa, w, off, out_dtype=torch.float32)
+    assert_near(y, *want, k + 128)
+    if len(sizes) == 1:
+        one = ma.Fp8Blocks(qw.data[0], qw.scale[0], "tile")
+        assert_near(ma.fp8_matmul(a, one), *want, k + 128)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,k,n", [
+    ([50, 0, 14], 136, 264), ([9], 64, 40), ([130, 40], 77, 111)])
+def test_fp8_gradients(sizes, k, n, dtype, device):
+    off = offsets_of(sizes, device)
+    a = randn(sum(sizes), k, seed=34, dtype=dtype, device=device)
+    w = randn(len(sizes), n, k, seed=35, dtype=dtype, device=device)
+    gy = randn(sum(sizes), n, seed=36, dtype=dtype, device=device)
+    a.requires_grad_()
+    w.requires_grad_()
+    da, dw = torch.autograd.grad(ma.fp8_matmul(a, w, off), (a, w), gy)
+    qg, qw = ma.quantize_fp8(gy), ma.quantize_fp8(w, "tile")
+    want = plain_rows(values_of(qg), values_of(qw), off)
+    assert da.dtype == dw.dtype == dtype
+    assert_near(da, *want, n + 128)
+    assert_near(dw, *plain_weights(gy, a, off), max(sizes))
+    da2, = torch.autograd.grad(ma.fp8_matmul(a, qw, off), a, gy)
+    assert torch.equal(da, da2)
+    assert torch.equal(qw.transpose().dequantize(),
+                       qw.dequantize().transpose(1, 2))
+    if len(sizes) == 1:
+        w1 = w.detach()[0].requires_grad_()
+        da, dw1 = torch.autograd.grad(ma.fp8_matmul(a, w1), (a, w1), gy)
+        assert torch.equal(dw1, dw[0]) and torch.equal(da, da2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_fp8_refusals(device):
+    a = torch.zeros(8, 256, dtype=torch.bfloat16, device=device)
+    w = torch.zeros(2, 16, 256, dtype=torch.bfloat16, device=device)
+    off = offsets_of([3, 5], device)
+    qa, qw = ma.quantize_fp8(a), ma.quantize_fp8(w, "tile")
+    for args in ((a, w), (a, w[0], off), (a[0], w, off), (a[:, :128], w, off),
+                 (qw, qw, off), (qa, ma.quantize_fp8(w, "row"), off),
+                 (a, w, off[:2]), (a.double(), w, off), (a.float(), w, off),
+                 (a, w, off.float())):
+        with pytest.raises((ValueError, TypeError)):
+            ma.fp8_matmul(*args)
+    with pytest.raises(ValueError):
+        ma.fp8_matmul(qa, w.clone().requires_grad_(), off)
+    with pytest.raises(ValueError):
+        ma.quantize_fp8(a, "column")
+    with pytest.raises(ValueError):
+        ma.quantize_fp8(a[0])
+    with pytest.raises(TypeError):
+        ma.quantize_fp8(a.double())
+    with pytest.raises(ValueError):
+        qa.transpose()
+    for data, scale, kind in (
+            (qa.data, qa.scale, "tile"), (qa.data, qa.scale.t(), "row"),
+            (qa.data, qa.scale, "both"),
+            (qa.data.t(), qa.scale, "row")):
+        with pytest.raises((ValueError, TypeError)):
+            ma.Fp8Blocks(data, scale, kind)
+    with pytest.raises(TypeError):
+        ma.Fp8Blocks(a, qa.scale, "row")
