@@ -59,6 +59,11 @@ bool aligned(const Tensor& t, int64_t ld, int64_t count) {
          (count <= 1 || ld * es % 16 == 0);
 }
 
+// Also a tile's 256 rows within 32 bits of its first one.
+bool fast_rows(const Tensor& t, int64_t ld, int64_t count) {
+  return aligned(t, ld, count) && ld * t.element_size() < (1 << 24);
+}
+
 void set_offsets(GroupedArgs& p, const c10::optional<Tensor>& offs,
                  const Tensor& a, int64_t groups) {
   if (!offs.has_value()) {
@@ -123,8 +128,8 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.gsb = E > 1 ? b.stride(0) : 0;
   p.splits = 1;
   p.out = type_of(out);
-  const bool fast = aligned(a, p.lda, T) &&
-                    aligned(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
+  const bool fast = fast_rows(a, p.lda, T) &&
+                    fast_rows(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
                     (bk || N % epc == 0);
   const int tile = choose_tile(T / E, T, N);
   launch_rows(p, ty, tile, bk, fast, stream_of(a));
@@ -163,7 +168,7 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.ldb = T > 1 ? b.stride(0) : 0;
   p.splits = 1;
   p.out = type_of(out);
-  const bool fast = aligned(a, p.lda, T) && aligned(b, p.ldb, T) &&
+  const bool fast = fast_rows(a, p.lda, T) && fast_rows(b, p.ldb, T) &&
                     M % epc == 0 && N % epc == 0;
   const int tile = choose_tile(M, T, N);
   const hipStream_t s = stream_of(a);
@@ -227,7 +232,7 @@ Tensor grouped_rows_fp8(Tensor a, Tensor asc, Tensor bt, Tensor bsc,
   p.splits = 1;
   p.out = type_of(c.scalar_type());
   p.accum = accum;
-  const bool fast = aligned(a, p.lda, T) && aligned(bt, p.ldb, N) &&
+  const bool fast = fast_rows(a, p.lda, T) && fast_rows(bt, p.ldb, N) &&
                     aligned(bt, p.gsb, E);
   launch_rows(p, GT_FP8, choose_tile(T / E, T, N), true, fast, stream_of(a));
   return c;

@@ -183,6 +183,7 @@ __device__ __forceinline__ bool find_row_tile(const GroupedArgs& p, int ntn,
 template <int TY, int R, int NT, bool KROWS>
 struct Side {
   typedef typename Elt<TY>::T E;
+  typedef i32x4 Regs[R * 8 / NT];
   static constexpr int ES = Elt<TY>::ES;
   static constexpr int EPC = 16 / ES;          // elements of a chunk
   static constexpr int BKE = 128 / ES;         // k of a tile
@@ -190,8 +191,8 @@ struct Side {
   static constexpr int CPR = R * ES / 16;      // R side: chunks of one k
   static_assert(R * 8 % NT == 0, "whole chunks for every thread");
 
-  const char* at[IT];  // where this thread's chunks of the first tile begin
-  const E* base;
+  u32 at[IT];        // this thread's chunks of a tile, bytes from `base`
+  const char* base;  // the operand's first row (R side: column) and k
   long ld;
   int row0, rlim, k0;
 
@@ -207,27 +208,28 @@ struct Side {
     }
   }
 
-  // Rows [row0, row0 + R) of which those below rlim exist (at least one).
+  // Rows [row0, row0 + R), of which those below rlim exist (at least one
+  // where `fast`), from k0 on.
   __device__ __forceinline__ void init(const void* b, long ld_, int row0_,
                                        int rlim_, int k0_, bool fast) {
-    base = (const E*)b;
     ld = ld_;
     row0 = row0_;
     rlim = rlim_;
     k0 = k0_;
+    base = (const char*)b +
+           (KROWS ? (long)row0 * ld + k0 : (long)k0 * ld + row0) * ES;
     if (!fast) return;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int id = i * NT + (int)threadIdx.x;
-      long e;
       if constexpr (KROWS) {
         const int row = id >> 3, c = (id & 7) ^ (row >> 1 & 7);
-        e = (long)min(row0 + row, rlim - 1) * ld + k0 + c * EPC;
+        at[i] = (u32)min(row, rlim - 1 - row0) * (u32)ld * ES + c * 16;
       } else {
         const int k = id / CPR, c = swz(id % CPR, k);
-        e = (long)(k0 + k) * ld + min(row0 + c * EPC, rlim - EPC);
+        at[i] = (u32)k * (u32)ld * ES +
+                (u32)min(c * EPC, rlim - EPC - row0) * ES;
       }
-      at[i] = (const char*)base + e * ES;
     }
   }
 
@@ -235,64 +237,48 @@ struct Side {
   // A row (R side: a chunk of rows) past the end reads the last one again;
   // what it makes is never stored.
   __device__ __forceinline__ void copy(char* lds, int tile) const {
-    const long step = (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
+    const char* s = base + (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
 #pragma unroll
     for (int i = 0; i < IT; ++i)
-      glds16(at[i] + step, lds + (i * NT + threadIdx.x) * 16);
+      glds16(s + at[i], lds + (i * NT + threadIdx.x) * 16);
   }
 
-  // Any tile: through registers, zeros outside of the rows and of k < klim.
-  __device__ __forceinline__ void gather(char* lds, int tile, int klim,
-                                         bool aligned) const {
+  // Any tile, any alignment: through registers, zeros outside of the rows
+  // and of k < klim.
+  __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile,
+                                       int klim) const {
+    const E* s0 = (const E*)base;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int id = i * NT + (int)threadIdx.x;
-      E v[EPC];
-#pragma unroll
-      for (int j = 0; j < EPC; ++j) v[j] = 0;
-      i32x4 w = {0, 0, 0, 0};
-      bool whole = false;
+      int n;  // elements of the chunk that exist
+      const E* s;
       if constexpr (KROWS) {
-        const int row = row0 + (id >> 3);
-        const int k = k0 + tile * BKE + ((id & 7) ^ ((id >> 3) >> 1 & 7)) * EPC;
-        const E* s = base + (long)row * ld + k;
-        if (row < rlim && k < klim) {
-          if (aligned && k + EPC <= klim) {
-            w = *(const i32x4*)s;
-            whole = true;
-          } else {
-#pragma unroll
-            for (int j = 0; j < EPC; ++j)
-              if (k + j < klim) v[j] = s[j];
-          }
-        }
+        const int row = id >> 3;
+        const int k = tile * BKE + ((id & 7) ^ (row >> 1 & 7)) * EPC;
+        n = row0 + row < rlim ? klim - k0 - k : 0;
+        s = s0 + (long)row * ld + k;
       } else {
-        const int kk = id / CPR, k = k0 + tile * BKE + kk;
-        const int row = row0 + swz(id % CPR, kk) * EPC;
-        const E* s = base + (long)k * ld + row;
-        if (k < klim && row < rlim) {
-          if (aligned && row + EPC <= rlim) {
-            w = *(const i32x4*)s;
-            whole = true;
-          } else {
-#pragma unroll
-            for (int j = 0; j < EPC; ++j)
-              if (row + j < rlim) v[j] = s[j];
-          }
-        }
+        const int k = tile * BKE + id / CPR;
+        const int row = swz(id % CPR, id / CPR) * EPC;
+        n = k0 + k < klim ? rlim - row0 - row : 0;
+        s = s0 + (long)k * ld + row;
       }
-      if (!whole) {
+      w[i] = i32x4{0, 0, 0, 0};
+      if (n >= EPC) {
+        __builtin_memcpy(&w[i], s, 16);  // global loads need no alignment
+      } else if (n > 0) {
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          u32 x = 0;
-#pragma unroll
-          for (int j = 0; j < 4 / ES; ++j)
-            x |= (u32)v[d * (4 / ES) + j] << (8 * ES * j);
-          w[d] = (int)x;
-        }
+        for (int j = 0; j < EPC; ++j)
+          if (j < n) w[i][j * ES / 4] |= (int)((u32)s[j] << (j * ES % 4 * 8));
       }
-      *(i32x4*)(lds + id * 16) = w;
     }
+  }
+
+  static __device__ __forceinline__ void put(char* lds, const i32x4 (&w)[IT]) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      *(i32x4*)(lds + (i * NT + threadIdx.x) * 16) = w[i];
   }
 
   // The chunk of the fragment of rows [row, row + 16) (row: a multiple of 16)
@@ -331,14 +317,105 @@ struct Side {
   }
 };
 
-// ---- the kernel ------------------------------------------------------------
+// ---- what a workgroup computes ---------------------------------------------
+
+struct Work {
+  int g;           // group (rows: -1 or E for rows of no group)
+  int m0, mend;    // first row and the end of the rows
+  int n0;
+  int kbeg, kend;  // what is summed
+};
+
+template <int TY, int BM, int BN, bool WEIGHTS>
+__device__ __forceinline__ bool locate(const GroupedArgs& p, Work* w) {
+  constexpr int BKE = 128 / Elt<TY>::ES;
+  const int ntn = (p.N + BN - 1) / BN;
+  if constexpr (WEIGHTS) {
+    // every XCD takes a share of every group: groups differ in length
+    const int ntm = (p.M + BM - 1) / BM, per = ntm * ntn;
+    w->g = blockIdx.x / per;
+    const int rem = (int)xcd_swizzle(blockIdx.x - w->g * per, per);
+    const int band = rem / (8 * ntn), r = rem - band * 8 * ntn;
+    const int wide = min(8, ntm - band * 8);
+    w->m0 = (band * 8 + r % wide) * BM;
+    w->n0 = r / wide * BN;
+    w->mend = p.M;
+    w->kbeg = bound_at(p, w->g + 1);
+    w->kend = max(w->kbeg, bound_at(p, w->g + 2));
+  } else {
+    RowTile t;
+    if (!find_row_tile<BM>(p, ntn, &t)) return false;
+    w->g = t.g;
+    w->m0 = t.m0;
+    w->mend = t.mend;
+    w->n0 = t.nt * BN;
+    w->kbeg = 0;
+    w->kend = t.g < 0 || t.g >= p.E ? 0 : p.K;
+  }
+  if (p.splits > 1) {  // an equal share of whole K tiles for each
+    const int tiles = (w->kend - w->kbeg + BKE - 1) / BKE;
+    const int share = (tiles + p.splits - 1) / p.splits;
+    const int lo = min(w->kend, w->kbeg + (int)blockIdx.y * share * BKE);
+    w->kend = min(w->kend, lo + share * BKE);
+    w->kbeg = lo;
+  }
+  // the same for all lanes, which only their owner can know
+  w->g = __builtin_amdgcn_readfirstlane(w->g);
+  w->m0 = __builtin_amdgcn_readfirstlane(w->m0);
+  w->mend = __builtin_amdgcn_readfirstlane(w->mend);
+  w->n0 = __builtin_amdgcn_readfirstlane(w->n0);
+  w->kbeg = __builtin_amdgcn_readfirstlane(w->kbeg);
+  w->kend = __builtin_amdgcn_readfirstlane(w->kend);
+  return true;
+}
+
+// Where results go. A lane holds four neighbouring n of one row.
+template <bool WEIGHTS> struct Results {
+  void* c;
+  int ty;
+  bool vec, accum;
+  long first;
+  int mend, n;
+
+  __device__ __forceinline__ Results(const GroupedArgs& p, const Work& w) {
+    const long rows = WEIGHTS ? (long)p.E * p.M : p.T;
+    c = p.part ? (void*)(p.part + blockIdx.y * rows * p.N) : p.c;
+    ty = p.part ? (int)GT_F32 : p.out;
+    vec = p.N % 4 == 0 && (u64)c % 16 == 0;
+    accum = p.accum;
+    first = WEIGHTS ? (long)w.g * p.M : 0;
+    mend = w.mend;
+    n = p.N;
+  }
+
+  // A 16 x 16 fragment at (row, col): lane l has row l & 15 and columns
+  // 4 (l >> 4) + 0..3.
+  __device__ __forceinline__ void put(int row, int col, f32x4 v) const {
+    const int lane = threadIdx.x & 63;
+    row += lane & 15;
+    col += (lane >> 4) * 4;
+    if (row >= mend || col >= n) return;
+    const long at = (first + row) * n + col;
+    const int have = min(4, n - col);
+    if (accum) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < have) v[q] += ((const float*)c)[at + q];
+    }
+    store4(c, at, ty, v, have, vec);
+  }
+};
+
+// ---- small and middle tiles ------------------------------------------------
 
 // BM x BN results a workgroup, its waves WM x WN. AK/BK: the operand has k
 // along its rows. WEIGHTS: the sum runs over a group's rows. FAST: rows (and
 // for an R side its length) are multiples of 16 bytes.
 //
 // Two LDS buffers: the copy of the next K tile runs under the products of
-// this one, with one barrier a tile.
+// this one, with one barrier a tile. Operands that are not FAST, and a last
+// tile that ends early, go through registers instead: loaded before the
+// products, put into LDS behind them.
 template <int TY, int BM, int BN, int WM, int WN, bool AK, bool BK,
           bool WEIGHTS, bool FAST>
 __global__ void __launch_bounds__(64 * WM * WN)
@@ -351,38 +428,8 @@ grouped_k(const GroupedArgs p) {
   constexpr int BUF = (BM + BN) * 128;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
-  const int ntn = (p.N + BN - 1) / BN;
-  int g, m0, mend, n0, kbeg, kend;
-  if constexpr (WEIGHTS) {
-    const int ntm = (p.M + BM - 1) / BM;
-    const int id = (int)xcd_swizzle(blockIdx.x, gridDim.x);
-    g = id / (ntm * ntn);
-    const int rem = id - g * ntm * ntn;
-    const int band = rem / (8 * ntn), r = rem - band * 8 * ntn;
-    const int wide = min(8, ntm - band * 8);
-    m0 = (band * 8 + r % wide) * BM;
-    n0 = r / wide * BN;
-    mend = p.M;
-    kbeg = bound_at(p, g + 1);
-    kend = max(kbeg, bound_at(p, g + 2));
-  } else {
-    RowTile t;
-    if (!find_row_tile<BM>(p, ntn, &t)) return;
-    g = t.g;
-    m0 = t.m0;
-    mend = t.mend;
-    n0 = t.nt * BN;
-    kbeg = 0;
-    kend = g < 0 || g >= p.E ? 0 : p.K;
-  }
-  const int split = blockIdx.y;
-  if (p.splits > 1) {  // an equal share of whole K tiles for each
-    const int tiles = (kend - kbeg + BKE - 1) / BKE;
-    const int share = (tiles + p.splits - 1) / p.splits;
-    const int lo = min(kend, kbeg + split * share * BKE);
-    kend = min(kend, lo + share * BKE);
-    kbeg = lo;
-  }
+  Work w;
+  if (!locate<TY, BM, BN, WEIGHTS>(p, &w)) return;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
@@ -393,9 +440,7 @@ grouped_k(const GroupedArgs p) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
 
-  SA sa;
-  SB sb;
-  const int depth = kend - kbeg;
+  const int depth = w.kend - w.kbeg;
   const int whole = depth / BKE, tiles = (depth + BKE - 1) / BKE;
 
   const float* asc = nullptr;
@@ -403,10 +448,11 @@ grouped_k(const GroupedArgs p) {
   int nb = 0;
   if constexpr (TY == GT_FP8) {
     nb = (p.N + 127) / 128;
-    asc = p.asc + (long)(kbeg / 128) * p.T;
-    bsc = p.bsc + ((long)g * ((p.K + 127) / 128) + kbeg / 128) * nb +
-          (n0 + wn) / 128;
-    if (n0 + wn >= p.N) bsc = p.bsc;  // a wave past the end: stores nothing
+    asc = p.asc + (long)(w.kbeg / 128) * p.T;
+    bsc = p.bsc;  // a wave past the last column stores nothing
+    if (w.n0 + wn < p.N)
+      bsc += ((long)w.g * ((p.K + 127) / 128) + w.kbeg / 128) * nb +
+             (w.n0 + wn) / 128;
   }
 
   auto products = [&](const char* lds, int tile) {
@@ -420,7 +466,7 @@ grouped_k(const GroupedArgs p) {
       i32x8 y[FM];
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int row = min(m0 + wm + i * 16 + (lane & 15), p.T - 1);
+        const int row = min(w.m0 + wm + i * 16 + (lane & 15), p.T - 1);
         sc[i] = asc[(long)tile * p.T + row] * s;
         y[i] = join8(SA::frag(la, wm + i * 16, 0),
                      SA::frag(la, wm + i * 16, 1));
@@ -455,52 +501,273 @@ grouped_k(const GroupedArgs p) {
   };
 
   if (tiles > 0) {
-    const char* bbase = (const char*)p.b +
-                        (WEIGHTS ? 0 : (long)g * p.gsb * ES);
-    sa.init(p.a, p.lda, m0, mend, kbeg, FAST && whole > 0);
-    sb.init(bbase, p.ldb, n0, p.N, kbeg, FAST && whole > 0);
-    auto fill = [&](int tile) {
-      char* lds = smem + (tile & 1) * BUF;
-      if (FAST && tile < whole) {
+    SA sa;
+    SB sb;
+    sa.init(p.a, p.lda, w.m0, w.mend, w.kbeg, FAST);
+    sb.init((const char*)p.b + (WEIGHTS ? 0 : (long)w.g * p.gsb * ES), p.ldb,
+            w.n0, p.N, w.kbeg, FAST);
+    const int fast = FAST ? whole : 0;  // tiles that go straight to LDS
+    typename SA::Regs ra;
+    typename SB::Regs rb;
+    auto begin = [&](int tile) {
+      if (tile < fast) {
+        char* lds = smem + (tile & 1) * BUF;
         sa.copy(lds, tile);
         sb.copy(lds + BM * 128, tile);
       } else {
-        sa.gather(lds, tile, kend, FAST);
-        sb.gather(lds + BM * 128, tile, kend, FAST);
+        sa.load(ra, tile, w.kend);
+        sb.load(rb, tile, w.kend);
       }
     };
-    fill(0);
+    auto end = [&](int tile) {
+      if (tile >= fast) {
+        char* lds = smem + (tile & 1) * BUF;
+        SA::put(lds, ra);
+        SB::put(lds + BM * 128, rb);
+      }
+    };
+    begin(0);
+    end(0);
     for (int t = 0; t < tiles; ++t) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (t + 1 < tiles) fill(t + 1);
+      if (t + 1 < tiles) begin(t + 1);
       products(smem + (t & 1) * BUF, t);
+      if (t + 1 < tiles) end(t + 1);
     }
   }
 
-  // results: lane l holds row l & 15, columns 4 (l >> 4) + 0..3
-  const long rows = WEIGHTS ? (long)p.E * p.M : p.T;
-  const long first = WEIGHTS ? (long)g * p.M : 0;
-  void* c = p.part ? (void*)(p.part + split * rows * p.N) : p.c;
-  const int ty = p.part ? (int)GT_F32 : p.out;
-  const bool vec = p.N % 4 == 0 && (u64)c % 16 == 0;
+  const Results<WEIGHTS> out(p, w);
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int row = m0 + wm + i * 16 + (lane & 15);
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (row < mend && n < p.N) {
-        const long at = (first + row) * p.N + n;
-        const int have = min(4, p.N - n);
-        f32x4 v = acc[j][i];
-        if (p.accum) {
+    for (int j = 0; j < FN; ++j)
+      out.put(w.m0 + wm + i * 16, w.n0 + wn + j * 16, acc[j][i]);
+}
+
+// ---- the large tile --------------------------------------------------------
+
+// 256 x 256 results, 8 waves, operands whose rows begin on 16 bytes. A K tile
+// is four halves of 16 KB: A0, A1 (rows), B0, B1 (columns). In each of four
+// phases all waves work on one 128 x 128 quarter, a 32 x 64 slice each, in the
+// order A0B0, A0B1, A1B1, A1B0, so that the halves are needed one after
+// another: while a tile is multiplied the next one's halves are copied in
+// that order, one a phase, and a phase ends with a wait that leaves the
+// younger copies in flight. The copies are never waited for to the last one
+// inside the loop. The second four waves have the higher priority: two waves
+// of a SIMD then take turns at the matrix unit instead of reading LDS at once.
+template <int TY, bool AK, bool BK, bool WEIGHTS>
+__global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
+  constexpr int ES = Elt<TY>::ES, BKE = 128 / ES;
+  typedef Side<TY, 128, 512, AK> SA;
+  typedef Side<TY, 128, 512, BK> SB;
+  constexpr int HALF = 128 * 128, BUF = 4 * HALF;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+
+  Work w;
+  if (!locate<TY, 256, 256, WEIGHTS>(p, &w)) return;
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int qr = (wave & 3) * 32, qc = (wave >> 2) * 64;
+
+  f32x4 acc[2][2][4][2];  // [row half][column half][columns][rows]
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < have) v[q] += ((const float*)c)[at + q];
-        }
-        store4(c, at, ty, v, have, vec);
-      }
+  for (int i = 0; i < 32; ++i) ((f32x4*)acc)[i] = f32x4{0, 0, 0, 0};
+
+  const int depth = w.kend - w.kbeg;
+  const int whole = depth / BKE;
+
+  // fp8: scales of the wave's rows in both halves; of its columns uniform
+  u32 arow[2][2];
+  const float* asc = nullptr;
+  const float* bsc[2] = {nullptr, nullptr};
+  float ra[2][2], rb[2];
+  int nb = 0;
+  if constexpr (TY == GT_FP8) {
+    nb = (p.N + 127) / 128;
+    const long kb = w.kbeg / 128;
+    asc = p.asc + kb * p.T;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        arow[h][i] =
+            min(w.m0 + h * 128 + qr + i * 16 + (lane & 15), p.T - 1);
+      bsc[h] = p.bsc + ((long)max(0, min(w.g, p.E - 1)) * ((p.K + 127) / 128) +
+                        kb) * nb + min(w.n0 / 128 + h, nb - 1);
     }
   }
+  auto load_scales = [&](int tile) {
+    if constexpr (TY == GT_FP8) {
+      const float* s = asc + (long)tile * p.T;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ra[h][i] = s[arow[h][i]];
+        rb[h] = bsc[h][(long)tile * nb];
+      }
+    }
+  };
+
+  i32x4 y[2][2], x[2][4];  // [half of k][fragments]
+  auto read_a = [&](const char* buf, int h) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        y[kk][i] = SA::frag(buf + h * HALF, qr + i * 16, kk);
+  };
+  auto read_b = [&](const char* buf, int h) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[kk][j] = SB::frag(buf + (2 + h) * HALF, qc + j * 16, kk);
+  };
+  float sa_[2][2], sb_[2];  // the scales of the tile that is multiplied
+  auto quarter = [&](int hm, int hn) {
+    if constexpr (TY == GT_FP8) {
+      float sc[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc[i] = sa_[hm][i] * sb_[hn];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 d = mma_fp8(join8(x[0][j], x[1][j]),
+                                  join8(y[0][i], y[1][i]),
+                                  f32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            acc[hm][hn][j][i][q] =
+                __builtin_fmaf(d[q], sc[i], acc[hm][hn][j][i][q]);
+        }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            acc[hm][hn][j][i] =
+                mma<TY>(x[kk][j], y[kk][i], acc[hm][hn][j][i]);
+    }
+  };
+  auto take_scales = [&]() {
+    if constexpr (TY == GT_FP8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sa_[h][0] = ra[h][0];
+        sa_[h][1] = ra[h][1];
+        sb_[h] = rb[h];
+      }
+    }
+  };
+
+  if (depth > 0) {
+    const char* b = (const char*)p.b +
+                    (WEIGHTS ? 0 : (long)w.g * p.gsb * ES);
+    SA a0, a1;
+    SB b0, b1;
+    // a half past the end takes its row from inside
+    a0.init(p.a, p.lda, w.m0, w.mend, w.kbeg, true);
+    b0.init(b, p.ldb, w.n0, p.N, w.kbeg, true);
+    a1.init(p.a, p.lda, w.m0 + 128 < w.mend ? w.m0 + 128 : w.m0, w.mend,
+            w.kbeg, true);
+    b1.init(b, p.ldb, w.n0 + 128 < p.N ? w.n0 + 128 : w.n0, p.N, w.kbeg,
+            true);
+
+    // vector memory operations of a lane in flight at each wait, oldest
+    // first (2 a half; S: the scales of fp8, 4 or more; ' = next tile):
+    //   end of phase 1: B1 A1 S' A0'        B1 has to be there
+    //   end of phase 2: A1 S' A0' B0'       A1 has to be there
+    //   end of phase 4: S' A0' B0' B1' A1'  A0' and B0' have to be there
+#define GB_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+    auto step = [&](auto more, int t) {
+      const char* cur = smem + (t & 1) * BUF;
+      char* nxt = smem + (~t & 1) * BUF;
+      take_scales();
+      read_a(cur, 0);
+      read_b(cur, 0);
+      if constexpr (more) {
+        load_scales(t + 1);
+        a0.copy(nxt, t + 1);
+      }
+      quarter(0, 0);
+      if constexpr (!more) GB_WAIT(2);
+      else if constexpr (TY == GT_FP8) GB_WAIT(8);
+      else GB_WAIT(4);
+      __builtin_amdgcn_s_barrier();
+      read_b(cur, 1);
+      if constexpr (more) b0.copy(nxt + 2 * HALF, t + 1);
+      quarter(0, 1);
+      if constexpr (!more) GB_WAIT(0);
+      else if constexpr (TY == GT_FP8) GB_WAIT(8);
+      else GB_WAIT(4);
+      __builtin_amdgcn_s_barrier();
+      read_a(cur, 1);
+      if constexpr (more) b1.copy(nxt + 3 * HALF, t + 1);
+      quarter(1, 1);
+      read_b(cur, 0);
+      if constexpr (more) a1.copy(nxt + HALF, t + 1);
+      quarter(1, 0);
+      if constexpr (more) GB_WAIT(4);
+      __builtin_amdgcn_s_barrier();
+    };
+    struct Yes { constexpr operator bool() const { return true; } };
+    struct No { constexpr operator bool() const { return false; } };
+
+    if (__builtin_amdgcn_readfirstlane(threadIdx.x) >= 256)
+      __builtin_amdgcn_s_setprio(1);
+    if (whole > 0) {
+      load_scales(0);
+      a0.copy(smem, 0);
+      b0.copy(smem + 2 * HALF, 0);
+      b1.copy(smem + 3 * HALF, 0);
+      a1.copy(smem + HALF, 0);
+      GB_WAIT(4);
+      __builtin_amdgcn_s_barrier();
+      for (int t = 0; t + 1 < whole; ++t) step(Yes{}, t);
+      step(No{}, whole - 1);
+    }
+#undef GB_WAIT
+    if (whole * BKE < depth) {  // what is left of k
+      __syncthreads();
+      typename SA::Regs r;
+      typename SB::Regs s;
+      a0.load(r, whole, w.kend);
+      SA::put(smem, r);
+      a1.load(r, whole, w.kend);
+      SA::put(smem + HALF, r);
+      b0.load(s, whole, w.kend);
+      SB::put(smem + 2 * HALF, s);
+      b1.load(s, whole, w.kend);
+      SB::put(smem + 3 * HALF, s);
+      load_scales(whole);
+      __syncthreads();
+      take_scales();
+      read_a(smem, 0);
+      read_b(smem, 0);
+      quarter(0, 0);
+      read_b(smem, 1);
+      quarter(0, 1);
+      read_a(smem, 1);
+      quarter(1, 1);
+      read_b(smem, 0);
+      quarter(1, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  const Results<WEIGHTS> out(p, w);
+#pragma unroll
+  for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          out.put(w.m0 + hm * 128 + qr + i * 16, w.n0 + hn * 128 + qc + j * 16,
+                  acc[hm][hn][j][i]);
 }

@@ -5,7 +5,7 @@
 extern "C" void launch_grouped_fp8(const GroupedArgs* p, int tile, int fast,
                                    hipStream_t s) {
   if (!fast) grouped_go<GT_FP8, 128, 128, 2, 2, true, true, false, false>(*p, s);
-  else if (tile == 2) grouped_go<GT_FP8, 256, 256, 4, 2, true, true, false, true>(*p, s);
+  else if (tile == 2) grouped_big_go<GT_FP8, true, true, false>(*p, s);
   else if (tile == 1) grouped_go<GT_FP8, 128, 128, 2, 2, true, true, false, true>(*p, s);
   else grouped_go<GT_FP8, 32, 128, 1, 4, true, true, false, true>(*p, s);
 }

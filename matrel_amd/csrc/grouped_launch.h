@@ -14,3 +14,13 @@ static void grouped_go(const GroupedArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
                      dim3(64 * WM * WN), lds, s, p);
 }
+
+template <int TY, bool AK, bool BK, bool WEIGHTS>
+static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
+  const long ntn = (p.N + 255) / 256;
+  const long ntm = WEIGHTS ? (long)p.E * ((p.M + 255) / 256)
+                           : p.T / 256 + p.E + 2;
+  auto k = grouped_big_k<TY, AK, BK, WEIGHTS>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
+                     dim3(512), 2 * 4 * 128 * 128, s, p);
+}
