@@ -16,7 +16,7 @@ extern "C" {
 void launch_grouped_bf16(const GroupedArgs*, int, int, int, int, hipStream_t);
 void launch_grouped_f16(const GroupedArgs*, int, int, int, int, hipStream_t);
 void launch_grouped_f32(const GroupedArgs*, int, int, int, int, hipStream_t);
-void launch_grouped_fp8(const GroupedArgs*, int, int, hipStream_t);
+void launch_grouped_fp8(const GroupedArgs*, int, int, int, hipStream_t);
 void launch_grouped_join(const float*, void*, long, int, int, hipStream_t);
 void launch_fp8_quantize_row(const void*, int, long, long, long, void*,
                              float*, int, hipStream_t);
@@ -79,15 +79,17 @@ void set_offsets(GroupedArgs& p, const c10::optional<Tensor>& offs,
   p.off64 = offs->scalar_type() == torch::kInt64;
 }
 
-// 2: 256 x 256, 1: 128 x 128, 0: 32 x 128
-int choose_tile(int64_t rows_each, int64_t M, int64_t N) {
-  if (rows_each > 128 && N > 128) return 2;
-  return rows_each > 32 ? 1 : 0;
+// The tile for a product of `each` rows a group on average: 2: 256 x 256,
+// 1: 128 x 128, 0: 32 x 128, -1, -2: 16 columns of 16, 32 rows.
+int choose_tile(int64_t each, int64_t N, bool skinny) {
+  if (skinny && each <= 32) return each <= 16 ? -1 : -2;
+  if (each > 128 && N > 128) return 2;
+  return each > 32 ? 1 : 0;
 }
 
 void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
-                 hipStream_t s) {
-  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, s);
+                 hipStream_t s, int aty = GT_FP8) {
+  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, aty, s);
   else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, fast, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, fast, s);
   else launch_grouped_f32(&p, tile, bk, 0, fast, s);
@@ -131,7 +133,7 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   const bool fast = fast_rows(a, p.lda, T) &&
                     fast_rows(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
                     (bk || N % epc == 0);
-  const int tile = choose_tile(T / E, T, N);
+  const int tile = choose_tile((T + E - 1) / E, N, bk);
   launch_rows(p, ty, tile, bk, fast, stream_of(a));
   return c;
 }
@@ -170,7 +172,7 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.out = type_of(out);
   const bool fast = fast_rows(a, p.lda, T) && fast_rows(b, p.ldb, T) &&
                     M % epc == 0 && N % epc == 0;
-  const int tile = choose_tile(M, T, N);
+  const int tile = choose_tile(M, N, false);
   const hipStream_t s = stream_of(a);
   if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, fast, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, fast, s);
@@ -179,26 +181,46 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   return c;
 }
 
-// c = a @ bt[group]^T of e4m3 operands: a [T, K] with scales [kb][T], bt
-// [E, N, K] with scales [E][kb][nb]. With `into` (f32, contiguous), the
-// product is written there, or added where `accum` is set.
-Tensor grouped_rows_fp8(Tensor a, Tensor asc, Tensor bt, Tensor bsc,
-                        c10::optional<Tensor> offs, at::ScalarType out,
-                        c10::optional<Tensor> into, bool accum) {
+std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x);
+
+// c = a @ bt[group]^T of e4m3 operands: a [T, K] with scales [kb][T], or a
+// wider a without scales that is quantized by rows, bt [E, N, K] with scales
+// [E][kb][nb]. With `into` (f32, contiguous), the product is written there,
+// or added where `accum` is set.
+Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
+                        Tensor bsc, c10::optional<Tensor> offs,
+                        at::ScalarType out, c10::optional<Tensor> into,
+                        bool accum) {
   TORCH_CHECK(a.is_cuda() && bt.device() == a.device() &&
-              asc.device() == a.device() && bsc.device() == a.device(),
-              "operands must be on one GPU");
+              bsc.device() == a.device(), "operands must be on one GPU");
   TORCH_CHECK(a.dim() == 2 && bt.dim() == 3 && a.size(1) == bt.size(2) &&
-              a.scalar_type() == torch::kFloat8_e4m3fn &&
-              bt.scalar_type() == torch::kFloat8_e4m3fn &&
-              a.is_contiguous() && bt.is_contiguous(),
+              bt.scalar_type() == torch::kFloat8_e4m3fn && bt.is_contiguous(),
               "operands do not match");
   const c10::hip::HIPGuard guard(a.device().index());
   const int64_t T = a.size(0), K = a.size(1), N = bt.size(1), E = bt.size(0);
   const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
-  TORCH_CHECK(asc.scalar_type() == torch::kFloat32 && asc.is_contiguous() &&
-              asc.dim() == 2 && asc.size(0) == kb && asc.size(1) == T,
-              "scales of a must be float32 [ceil(K/128), rows]");
+  int tile = choose_tile(E ? (T + E - 1) / E : 0, N, true);
+  int aty = GT_FP8;
+  Tensor asc;
+  if (a_scales.has_value()) {
+    asc = *a_scales;
+    TORCH_CHECK(a.scalar_type() == torch::kFloat8_e4m3fn &&
+                a.is_contiguous(), "a with scales must be contiguous e4m3");
+    TORCH_CHECK(asc.device() == a.device() &&
+                asc.scalar_type() == torch::kFloat32 && asc.is_contiguous() &&
+                asc.dim() == 2 && asc.size(0) == kb && asc.size(1) == T,
+                "scales of a must be float32 [ceil(K/128), rows]");
+  } else {
+    TORCH_CHECK(K <= 1 || a.stride(1) == 1, "rows of a must be contiguous");
+    aty = type_of(a.scalar_type());
+    TORCH_CHECK(aty != GT_FP8, "e4m3 operands need scales");
+    // few 16-bit rows are quantized on the way into the product: the launch
+    // saved costs more than the conversion that every 16 columns repeat
+    if (tile != -1 || aty == GT_F32) {
+      std::tie(a, asc) = fp8_quantize_row(a);
+      aty = GT_FP8;
+    }
+  }
   TORCH_CHECK(bsc.scalar_type() == torch::kFloat32 && bsc.is_contiguous() &&
               bsc.dim() == 3 && bsc.size(0) == E && bsc.size(1) == kb &&
               bsc.size(2) == nb,
@@ -224,9 +246,9 @@ Tensor grouped_rows_fp8(Tensor a, Tensor asc, Tensor bt, Tensor bsc,
   p.a = a.data_ptr();
   p.b = bt.data_ptr();
   p.c = c.data_ptr();
-  p.asc = asc.data_ptr<float>();
+  p.asc = asc.defined() ? asc.data_ptr<float>() : nullptr;
   p.bsc = bsc.data_ptr<float>();
-  p.lda = T > 1 ? K : 0;
+  p.lda = T > 1 ? a.stride(0) : 0;
   p.ldb = N > 1 ? K : 0;
   p.gsb = E > 1 ? N * K : 0;
   p.splits = 1;
@@ -234,7 +256,7 @@ Tensor grouped_rows_fp8(Tensor a, Tensor asc, Tensor bt, Tensor bsc,
   p.accum = accum;
   const bool fast = fast_rows(a, p.lda, T) && fast_rows(bt, p.ldb, N) &&
                     aligned(bt, p.gsb, E);
-  launch_rows(p, GT_FP8, choose_tile(T / E, T, N), true, fast, stream_of(a));
+  launch_rows(p, GT_FP8, tile, true, fast, stream_of(a), aty);
   return c;
 }
 

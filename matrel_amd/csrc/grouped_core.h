@@ -118,40 +118,54 @@ __device__ __forceinline__ int bound_at(const GroupedArgs& p, int i) {
 }
 
 struct RowTile {
-  int g;     // group, -1 or E: rows of no group
+  int g;     // group, E or more: rows of no group
   int m0;    // first row
   int mend;  // end of the group's rows
   int nt;    // tile along n
 };
 
-// Tile `id` of the tiles of all ranges, each cut into BM rows x ntn tiles.
-// Neighbouring ids are kept within an 8-row-tile wide band of one group, so
-// that the workgroups of one XCD share both operands in its L2.
+// Inclusive prefix sum over the wave.
+__device__ __forceinline__ int wave_sum(int x) {
+#define STEP(ctrl, rows) \
+  x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false)
+  STEP(0x111, 0xf);  // from 1, 2, 4, 8 lanes before, within 16
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);  // lane 15 to the next 16, lane 31 to the next 32
+  STEP(0x143, 0xc);
+#undef STEP
+  return x;
+}
+
+// Tile `id` of the tiles of all ranges, each cut into BM rows x ntn tiles:
+// the groups', then those of the head and the tail. Neighbouring ids are kept
+// within an 8-row-tile wide band of one group, so that the workgroups of one
+// XCD share both operands in its L2.
 template <int BM>
 __device__ __forceinline__ bool find_row_tile(const GroupedArgs& p, int ntn,
                                               RowTile* out) {
   const int lane = threadIdx.x & 63;
-  const int nv = p.E + 2;
-  int total = 0, inc = 0, cnt = 0, lo = 0, hi = 0;
-  auto scan = [&](int base) {
+  int inc = 0, cnt = 0, lo = 0, hi = 0;
+  auto scan = [&](int base) {  // groups, or (E, E + 1): head and tail
     const int v = base + lane;
     lo = hi = 0;
-    if (v < nv) {
-      lo = bound_at(p, v);
-      hi = bound_at(p, v + 1);
-      if (hi < lo) hi = lo;
+    if (v < p.E) {
+      lo = bound_at(p, v + 1);
+      hi = bound_at(p, v + 2);
+    } else if (v < p.E + 2) {
+      lo = v == p.E ? 0 : bound_at(p, p.E + 1);
+      hi = v == p.E ? bound_at(p, 1) : p.T;
     }
+    if (hi < lo) hi = lo;
     cnt = (hi - lo + BM - 1) / BM * ntn;
-    inc = cnt;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      int t = __shfl_up(inc, d);
-      if (lane >= d) inc += t;
-    }
+    inc = wave_sum(cnt);
   };
+  const int nv = p.E + 2;
+  int total = 0;
   for (int base = 0; base < nv; base += 64) {
     scan(base);
-    total += __shfl(inc, 63);
+    total += __builtin_amdgcn_readlane(inc, 63);
   }
   if ((int)blockIdx.x >= total) return false;
   const int id = (int)xcd_swizzle(blockIdx.x, (u32)total);
@@ -161,18 +175,20 @@ __device__ __forceinline__ bool find_row_tile(const GroupedArgs& p, int ntn,
     const u64 m = __ballot(before + inc > id);
     if (m) {
       const int at = __ffsll((unsigned long long)m) - 1;
-      const int first = before + __shfl(inc, at) - __shfl(cnt, at);
-      const int s = __shfl(lo, at), e = __shfl(hi, at);
+      const int first = before + __builtin_amdgcn_readlane(inc, at) -
+                        __builtin_amdgcn_readlane(cnt, at);
+      const int s = __builtin_amdgcn_readlane(lo, at);
+      const int e = __builtin_amdgcn_readlane(hi, at);
       const int rem = id - first, mtc = (e - s + BM - 1) / BM;
       const int band = rem / (8 * ntn), r = rem - band * 8 * ntn;
       const int wide = min(8, mtc - band * 8);
-      out->g = base + at - 1;
+      out->g = base + at;
       out->m0 = s + (band * 8 + r % wide) * BM;
       out->mend = e;
       out->nt = r / wide;
       return true;
     }
-    before += __shfl(inc, 63);
+    before += __builtin_amdgcn_readlane(inc, 63);
   }
   return false;
 }
@@ -235,12 +251,30 @@ struct Side {
 
   // Whole tiles of operands whose rows begin on 16 bytes: straight to LDS.
   // A row (R side: a chunk of rows) past the end reads the last one again;
-  // what it makes is never stored.
-  __device__ __forceinline__ void copy(char* lds, int tile) const {
+  // what it makes is never stored. `lds`: an offset from smem.
+  __device__ __forceinline__ void copy(char* smem, u32 lds, int tile) const {
     const char* s = base + (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
+    if constexpr (ES != 1) {
+      const u64 v = (u64)s;
+      s = (const char*)((u64)(u32)__builtin_amdgcn_readfirstlane((u32)v) |
+                        (u64)(u32)__builtin_amdgcn_readfirstlane(
+                            (u32)(v >> 32)) << 32);
+    }
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
-      glds16(s + at[i], lds + (i * NT + threadIdx.x) * 16);
+    for (int i = 0; i < IT; ++i) {
+      if constexpr (ES == 1) {
+        glds16(s + at[i], smem + lds + (i * NT + threadIdx.x) * 16);
+      } else {
+        // the same instruction by hand: the compiler, which knows these
+        // copies, waits for all of them before each transposing read
+        const u32 to = __builtin_amdgcn_readfirstlane(
+            (u32)(uintptr_t)(__attribute__((address_space(3))) char*)smem +
+            lds + (i * NT + (threadIdx.x & ~63u)) * 16);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\t"
+                     "global_load_lds_dwordx4 %0, %1"
+                     :: "v"(at[i]), "s"(s), "s"(to));
+      }
+    }
   }
 
   // Any tile, any alignment: through registers, zeros outside of the rows
@@ -320,7 +354,7 @@ struct Side {
 // ---- what a workgroup computes ---------------------------------------------
 
 struct Work {
-  int g;           // group (rows: -1 or E for rows of no group)
+  int g;           // group (rows: E or more for rows of no group)
   int m0, mend;    // first row and the end of the rows
   int n0;
   int kbeg, kend;  // what is summed
@@ -350,7 +384,7 @@ __device__ __forceinline__ bool locate(const GroupedArgs& p, Work* w) {
     w->mend = t.mend;
     w->n0 = t.nt * BN;
     w->kbeg = 0;
-    w->kend = t.g < 0 || t.g >= p.E ? 0 : p.K;
+    w->kend = t.g >= p.E ? 0 : p.K;
   }
   if (p.splits > 1) {  // an equal share of whole K tiles for each
     const int tiles = (w->kend - w->kbeg + BKE - 1) / BKE;
@@ -412,11 +446,12 @@ template <bool WEIGHTS> struct Results {
 // along its rows. WEIGHTS: the sum runs over a group's rows. FAST: rows (and
 // for an R side its length) are multiples of 16 bytes.
 //
-// Two LDS buffers: the copy of the next K tile runs under the products of
-// this one, with one barrier a tile. Operands that are not FAST, and a last
-// tile that ends early, go through registers instead: loaded before the
-// products, put into LDS behind them.
-template <int TY, int BM, int BN, int WM, int WN, bool AK, bool BK,
+// D LDS stages: the copies of D - 1 K tiles are on their way at a time, since
+// a tile's products are shorter than the way to memory; one barrier a tile.
+// Operands that are not FAST, and a last tile that ends early, go through
+// registers instead: loaded before the products of the tile before, put into
+// LDS behind them.
+template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
           bool WEIGHTS, bool FAST>
 __global__ void __launch_bounds__(64 * WM * WN)
 grouped_k(const GroupedArgs p) {
@@ -425,7 +460,11 @@ grouped_k(const GroupedArgs p) {
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Side<TY, BM, NT, AK> SA;
   typedef Side<TY, BN, NT, BK> SB;
-  constexpr int BUF = (BM + BN) * 128;
+  // fp8: scales of BM rows, then of the columns, 64 a wave
+  constexpr int SCALES = TY == GT_FP8 ? NT * 4 : 0;
+  static_assert(!SCALES || BM + 64 <= NT, "a wave is left for the columns");
+  constexpr int STAGE = (BM + BN) * 128 + SCALES;
+  constexpr int OPS = SA::IT + SB::IT + (SCALES ? 1 : 0);  // copies a stage
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   Work w;
@@ -443,31 +482,30 @@ grouped_k(const GroupedArgs p) {
   const int depth = w.kend - w.kbeg;
   const int whole = depth / BKE, tiles = (depth + BKE - 1) / BKE;
 
-  const float* asc = nullptr;
-  const float* bsc = nullptr;
-  int nb = 0;
+  const float* scale = nullptr;  // this thread's, of the first tile
+  int scale_step = 0;
   if constexpr (TY == GT_FP8) {
-    nb = (p.N + 127) / 128;
-    asc = p.asc + (long)(w.kbeg / 128) * p.T;
-    bsc = p.bsc;  // a wave past the last column stores nothing
-    if (w.n0 + wn < p.N)
-      bsc += ((long)w.g * ((p.K + 127) / 128) + w.kbeg / 128) * nb +
-             (w.n0 + wn) / 128;
+    const int nb = (p.N + 127) / 128;
+    const long kb = w.kbeg / 128;
+    const bool rows = tid < BM;
+    scale = rows ? p.asc + kb * p.T + min(w.m0 + tid, p.T - 1)
+                 : p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
+                            kb) * nb + w.n0 / 128;
+    scale_step = rows ? p.T : nb;
   }
 
-  auto products = [&](const char* lds, int tile) {
+  auto products = [&](const char* lds) {
     const char* la = lds;
     const char* lb = lds + BM * 128;
     if constexpr (TY == GT_FP8) {
       // a K tile is one block of scales: its products are summed apart and
-      // join the f32 sum with one multiply-add
-      const float s = bsc[(long)tile * nb];
-      float sc[FM];
+      // join the f32 sum with one multiply-add. BN <= 128: one block of b
+      const float* sc = (const float*)(lds + (BM + BN) * 128);
+      float s[FM];
       i32x8 y[FM];
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int row = min(w.m0 + wm + i * 16 + (lane & 15), p.T - 1);
-        sc[i] = asc[(long)tile * p.T + row] * s;
+        s[i] = sc[wm + i * 16 + (lane & 15)] * sc[BM];
         y[i] = join8(SA::frag(la, wm + i * 16, 0),
                      SA::frag(la, wm + i * 16, 1));
       }
@@ -480,7 +518,7 @@ grouped_k(const GroupedArgs p) {
           const f32x4 d = mma_fp8(x, y[i], f32x4{0, 0, 0, 0});
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            acc[j][i][q] = __builtin_fmaf(d[q], sc[i], acc[j][i][q]);
+            acc[j][i][q] = __builtin_fmaf(d[q], s[i], acc[j][i][q]);
         }
       }
     } else {
@@ -507,33 +545,52 @@ grouped_k(const GroupedArgs p) {
     sb.init((const char*)p.b + (WEIGHTS ? 0 : (long)w.g * p.gsb * ES), p.ldb,
             w.n0, p.N, w.kbeg, FAST);
     const int fast = FAST ? whole : 0;  // tiles that go straight to LDS
+    int next = 0, to = 0;               // the next copy and its stage
+    auto copy = [&]() {
+      const u32 lds = to * STAGE;
+      if constexpr (SCALES)
+        glds4(scale + (long)next * scale_step,
+              smem + lds + (BM + BN) * 128 + tid * 4);
+      sa.copy(smem, lds, next);
+      sb.copy(smem, lds + BM * 128, next);
+      ++next;
+      to = to == D - 1 ? 0 : to + 1;
+    };
     typename SA::Regs ra;
     typename SB::Regs rb;
-    auto begin = [&](int tile) {
-      if (tile < fast) {
-        char* lds = smem + (tile & 1) * BUF;
-        sa.copy(lds, tile);
-        sb.copy(lds + BM * 128, tile);
-      } else {
-        sa.load(ra, tile, w.kend);
-        sb.load(rb, tile, w.kend);
-      }
+    float rs = 0;
+    auto load = [&](int tile) {
+      if constexpr (SCALES) rs = scale[(long)tile * scale_step];
+      sa.load(ra, tile, w.kend);
+      sb.load(rb, tile, w.kend);
     };
-    auto end = [&](int tile) {
-      if (tile >= fast) {
-        char* lds = smem + (tile & 1) * BUF;
-        SA::put(lds, ra);
-        SB::put(lds + BM * 128, rb);
-      }
+    auto put = [&](int stage) {
+      char* lds = smem + stage * STAGE;
+      SA::put(lds, ra);
+      SB::put(lds + BM * 128, rb);
+      if constexpr (SCALES) ((float*)(lds + (BM + BN) * 128))[tid] = rs;
     };
-    begin(0);
-    end(0);
+    for (int i = 0; i < D - 1 && i < fast; ++i) copy();
+    if (fast == 0) {
+      load(0);
+      put(0);
+    }
+    int stage = 0;
     for (int t = 0; t < tiles; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (t + 1 < tiles) begin(t + 1);
-      products(smem + (t & 1) * BUF, t);
-      if (t + 1 < tiles) end(t + 1);
+      // tile t is there when no more than the D - 2 behind it are missing
+      if (FAST && next < fast)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * OPS) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      if (next < fast) copy();
+      const int after = stage == D - 1 ? 0 : stage + 1;
+      const bool regs = t + 1 < tiles && t + 1 >= fast;
+      if (regs) load(t + 1);
+      products(smem + stage * STAGE);
+      if (regs) put(after);
+      stage = after;
     }
   }
 
@@ -593,7 +650,7 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       for (int i = 0; i < 2; ++i)
         arow[h][i] =
             min(w.m0 + h * 128 + qr + i * 16 + (lane & 15), p.T - 1);
-      bsc[h] = p.bsc + ((long)max(0, min(w.g, p.E - 1)) * ((p.K + 127) / 128) +
+      bsc[h] = p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
                         kb) * nb + min(w.n0 / 128 + h, nb - 1);
     }
   }
@@ -677,6 +734,16 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     b1.init(b, p.ldb, w.n0 + 128 < p.N ? w.n0 + 128 : w.n0, p.N, w.kbeg,
             true);
 
+    // Groups start at different K tiles: rows of many kilobytes lie a power of
+    // two apart, and all XCDs, each in its own group, would read the same
+    // columns, hence the same memory channels, at the same time. The order of
+    // a sum depends on its group alone.
+    const int turn = WEIGHTS ? 0 : (int)((long)whole * (w.g & 7) / 8);
+    auto at = [&](int t) {
+      t += turn;
+      return t >= whole ? t - whole : t;
+    };
+
     // vector memory operations of a lane in flight at each wait, oldest
     // first (2 a half; S: the scales of fp8, 4 or more; ' = next tile):
     //   end of phase 1: B1 A1 S' A0'        B1 has to be there
@@ -685,13 +752,13 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
 #define GB_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
     auto step = [&](auto more, int t) {
       const char* cur = smem + (t & 1) * BUF;
-      char* nxt = smem + (~t & 1) * BUF;
+      const u32 nxt = (~t & 1) * BUF;
       take_scales();
       read_a(cur, 0);
       read_b(cur, 0);
       if constexpr (more) {
-        load_scales(t + 1);
-        a0.copy(nxt, t + 1);
+        load_scales(at(t + 1));
+        a0.copy(smem, nxt, at(t + 1));
       }
       quarter(0, 0);
       if constexpr (!more) GB_WAIT(2);
@@ -699,19 +766,21 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       else GB_WAIT(4);
       __builtin_amdgcn_s_barrier();
       read_b(cur, 1);
-      if constexpr (more) b0.copy(nxt + 2 * HALF, t + 1);
+      if constexpr (more) b0.copy(smem, nxt + 2 * HALF, at(t + 1));
       quarter(0, 1);
       if constexpr (!more) GB_WAIT(0);
       else if constexpr (TY == GT_FP8) GB_WAIT(8);
       else GB_WAIT(4);
       __builtin_amdgcn_s_barrier();
       read_a(cur, 1);
-      if constexpr (more) b1.copy(nxt + 3 * HALF, t + 1);
+      if constexpr (more) b1.copy(smem, nxt + 3 * HALF, at(t + 1));
       quarter(1, 1);
       read_b(cur, 0);
-      if constexpr (more) a1.copy(nxt + HALF, t + 1);
+      if constexpr (more) a1.copy(smem, nxt + HALF, at(t + 1));
       quarter(1, 0);
+      // every read of this buffer is back too, before it is copied into
       if constexpr (more) GB_WAIT(4);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
     };
     struct Yes { constexpr operator bool() const { return true; } };
@@ -720,11 +789,11 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     if (__builtin_amdgcn_readfirstlane(threadIdx.x) >= 256)
       __builtin_amdgcn_s_setprio(1);
     if (whole > 0) {
-      load_scales(0);
-      a0.copy(smem, 0);
-      b0.copy(smem + 2 * HALF, 0);
-      b1.copy(smem + 3 * HALF, 0);
-      a1.copy(smem + HALF, 0);
+      load_scales(at(0));
+      a0.copy(smem, 0, at(0));
+      b0.copy(smem, 2 * HALF, at(0));
+      b1.copy(smem, 3 * HALF, at(0));
+      a1.copy(smem, HALF, at(0));
       GB_WAIT(4);
       __builtin_amdgcn_s_barrier();
       for (int t = 0; t + 1 < whole; ++t) step(Yes{}, t);
@@ -760,6 +829,41 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
   }
 
   const Results<WEIGHTS> out(p, w);
+  if (out.ty != GT_F32 && out.n % 8 == 0 && (u64)out.c % 16 == 0) {
+    // 16-bit results turn round in LDS, so that 32 lanes store 512 bytes of
+    // a row: 4 KB rows x 8-byte pieces from registers reach half the rate
+    __syncthreads();
+#pragma unroll
+    for (int hm = 0; hm < 2; ++hm)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = hm * 128 + qr + i * 16 + (lane & 15);
+#pragma unroll
+        for (int hn = 0; hn < 2; ++hn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c8 = (hn * 128 + qc + j * 16 + (lane >> 4) * 4) / 4;
+            const f32x4 v = acc[hm][hn][j][i];
+            const u32 lo = f32_to_bits16(v[0], out.ty) |
+                           (u32)f32_to_bits16(v[1], out.ty) << 16;
+            const u32 hi = f32_to_bits16(v[2], out.ty) |
+                           (u32)f32_to_bits16(v[3], out.ty) << 16;
+            *(uint2*)(smem + row * 512 +
+                      ((c8 ^ (row & 15) << 1) << 3)) = make_uint2(lo, hi);
+          }
+      }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int row = i * 16 + (threadIdx.x >> 5), c = threadIdx.x & 31;
+      const i32x4 v =
+          *(const i32x4*)(smem + row * 512 + ((c ^ (row & 15)) << 4));
+      const int r = w.m0 + row, n = w.n0 + c * 8;
+      if (r < out.mend && n < out.n)
+        *(i32x4*)((unsigned short*)out.c + (out.first + r) * out.n + n) = v;
+    }
+    return;
+  }
 #pragma unroll
   for (int hm = 0; hm < 2; ++hm)
 #pragma unroll

@@ -147,13 +147,17 @@ def quantize_fp8(x: torch.Tensor, kind: str = "row") -> Fp8Blocks:
     return Fp8Blocks(q.view(n, r, c), s, kind)
 
 
-def _product(a: Fp8Blocks, bt: Fp8Blocks, offsets, out_dtype):
-    """a @ bt[group]^T; bt [groups, n, k]."""
-    if not use_hip(a.data):
-        return rows_product(a.dequantize(), bt.dequantize().transpose(1, 2),
+def _product(a, bt: Fp8Blocks, offsets, out_dtype):
+    """a @ bt[group]^T; a: blocks, or values to be quantized; bt [groups, n,
+    k]."""
+    blocks = isinstance(a, Fp8Blocks)
+    if not use_hip(bt.data):
+        q = a if blocks else _cpu_quantize(a, "row")
+        return rows_product(q.dequantize(), bt.dequantize().transpose(1, 2),
                             offsets, out_dtype)
     return require_ext().grouped_rows_fp8(
-        a.data, a.scale, bt.data, bt.scale,
+        a.data if blocks else rows_contiguous(a),
+        a.scale if blocks else None, bt.data, bt.scale,
         None if offsets is None else offsets.contiguous(), out_dtype, None,
         False)
 
@@ -188,7 +192,7 @@ class _Fp8Matmul(torch.autograd.Function):
         ctx.a_dtype = a.dtype
         ctx.save_for_backward(
             a if ctx.needs_input_grad[1] else None, offsets)
-        return _product(quantize_fp8(a), q, offsets, out_dtype)
+        return _product(a, q, offsets, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -198,7 +202,7 @@ class _Fp8Matmul(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             turned = ctx.turned if ctx.turned is not None \
                 else ctx.frozen.transpose()
-            da = _product(quantize_fp8(grad), turned, offsets, ctx.a_dtype)
+            da = _product(grad, turned, offsets, ctx.a_dtype)
         if ctx.needs_input_grad[1]:
             # in the operands' own type: the sum runs over rows, along which
             # neither has its scales

@@ -5,6 +5,7 @@
 gfx950 (MI355X) only - no multi-arch fatbins, no CUDA path.
 """
 
+import glob
 import os
 
 from setuptools import setup
@@ -35,6 +36,15 @@ sources = [
     os.path.join(CSRC, "grouped_f32.hip"),
     os.path.join(CSRC, "grouped_fp8.hip"),
 ]
+
+# Objects do not know the headers they were made from: those older than the
+# newest header are made again.
+headers = max(os.path.getmtime(h) for h in glob.glob(
+    os.path.join(CSRC, "*.h")) if not h.endswith("_hip.h"))
+for obj in glob.glob(os.path.join(ROOT, "build", "temp*", "**", "*.o"),
+                     recursive=True):
+    if os.path.getmtime(obj) < headers:
+        os.remove(obj)
 
 setup(
     name="matrel_amd",
