@@ -59,9 +59,11 @@ bool aligned(const Tensor& t, int64_t ld, int64_t count) {
          (count <= 1 || ld * es % 16 == 0);
 }
 
-// Also a tile's 256 rows within 32 bits of its first one.
-bool fast_rows(const Tensor& t, int64_t ld, int64_t count) {
-  return aligned(t, ld, count) && ld * t.element_size() < (1 << 24);
+// A row of `len` elements holds 16 bytes, and a tile's 256 rows lie within 32
+// bits of its first one.
+bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
+  return len * t.element_size() >= 16 &&
+         ld * t.element_size() < (1 << 24);
 }
 
 void set_offsets(GroupedArgs& p, const c10::optional<Tensor>& offs,
@@ -130,8 +132,10 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.gsb = E > 1 ? b.stride(0) : 0;
   p.splits = 1;
   p.out = type_of(out);
-  const bool fast = fast_rows(a, p.lda, T) &&
-                    fast_rows(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
+  p.near_a = near_rows(a, p.lda, K);
+  p.near_b = near_rows(b, p.ldb, bk ? K : N);
+  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
+                    aligned(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
                     (bk || N % epc == 0);
   const int tile = choose_tile((T + E - 1) / E, N, bk);
   launch_rows(p, ty, tile, bk, fast, stream_of(a));
@@ -170,7 +174,10 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.ldb = T > 1 ? b.stride(0) : 0;
   p.splits = 1;
   p.out = type_of(out);
-  const bool fast = fast_rows(a, p.lda, T) && fast_rows(b, p.ldb, T) &&
+  p.near_a = near_rows(a, p.lda, M);
+  p.near_b = near_rows(b, p.ldb, N);
+  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
+                    aligned(b, p.ldb, T) &&
                     M % epc == 0 && N % epc == 0;
   const int tile = choose_tile(M, N, false);
   const hipStream_t s = stream_of(a);
@@ -254,8 +261,10 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   p.splits = 1;
   p.out = type_of(c.scalar_type());
   p.accum = accum;
-  const bool fast = fast_rows(a, p.lda, T) && fast_rows(bt, p.ldb, N) &&
-                    aligned(bt, p.gsb, E);
+  p.near_a = near_rows(a, p.lda, K);
+  p.near_b = near_rows(bt, p.ldb, K);
+  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
+                    aligned(bt, p.ldb, N) && aligned(bt, p.gsb, E);
   launch_rows(p, GT_FP8, tile, true, fast, stream_of(a), aty);
   return c;
 }

@@ -224,17 +224,17 @@ struct Side {
     }
   }
 
-  // Rows [row0, row0 + R), of which those below rlim exist (at least one
-  // where `fast`), from k0 on.
+  // Rows [row0, row0 + R), of which those below rlim exist (at least one),
+  // from k0 on. A row (R side: a chunk of rows) past the end reads the last
+  // one again; what it makes is never stored.
   __device__ __forceinline__ void init(const void* b, long ld_, int row0_,
-                                       int rlim_, int k0_, bool fast) {
+                                       int rlim_, int k0_) {
     ld = ld_;
     row0 = row0_;
     rlim = rlim_;
     k0 = k0_;
     base = (const char*)b +
            (KROWS ? (long)row0 * ld + k0 : (long)k0 * ld + row0) * ES;
-    if (!fast) return;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int id = i * NT + (int)threadIdx.x;
@@ -244,14 +244,13 @@ struct Side {
       } else {
         const int k = id / CPR, c = swz(id % CPR, k);
         at[i] = (u32)k * (u32)ld * ES +
-                (u32)min(c * EPC, rlim - EPC - row0) * ES;
+                (u32)(min(c * EPC, rlim - EPC - row0) * ES);
       }
     }
   }
 
   // Whole tiles of operands whose rows begin on 16 bytes: straight to LDS.
-  // A row (R side: a chunk of rows) past the end reads the last one again;
-  // what it makes is never stored. `lds`: an offset from smem.
+  // `lds`: an offset from smem.
   __device__ __forceinline__ void copy(char* smem, u32 lds, int tile) const {
     const char* s = base + (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
     if constexpr (ES != 1) {
@@ -277,12 +276,74 @@ struct Side {
     }
   }
 
-  // Any tile, any alignment: through registers, zeros outside of the rows
-  // and of k < klim.
-  __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile,
-                                       int klim) const {
-    const E* s0 = (const E*)base;
+  // Any tile, any alignment: through registers, zeros for k >= klim.
+  // Loads stay free of branches (one inside would wait for the one before):
+  // a chunk that ends early is read from further in front and shifted.
+  // near: a row has at least a chunk, and offsets fit 32 bits.
+  __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile, int klim,
+                                       bool near) const {
+    if (!near) {
+      load_slowly(w, tile, klim);
+      return;
+    }
+    const int k1 = klim - k0 - tile * BKE;  // k of the tile that exist
+    const char* s = base + (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
+    if (k1 >= BKE) {
 #pragma unroll
+      for (int i = 0; i < IT; ++i)  // global loads need no alignment
+        __builtin_memcpy(&w[i], s + at[i], 16);
+    } else {
+      long back[IT];
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int id = i * NT + (int)threadIdx.x;
+        if constexpr (KROWS)
+          back[i] = max(0, (((id & 7) ^ (id >> 4 & 7)) + 1) * EPC - k1) * ES;
+        else
+          back[i] = max(0, id / CPR + 1 - k1) * ld * ES;
+      }
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+        __builtin_memcpy(&w[i], s + at[i] - back[i], 16);
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        if constexpr (KROWS) w[i] = shifted(w[i], (int)back[i]);
+        else if ((i * NT + (int)threadIdx.x) / CPR >= k1)
+          w[i] = i32x4{0, 0, 0, 0};
+      }
+    }
+    if constexpr (!KROWS) {
+      if (row0 + R > rlim) {  // the last chunk of rows may be a part
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int id = i * NT + (int)threadIdx.x;
+          const int c = swz(id % CPR, id / CPR) * EPC;
+          w[i] = shifted(w[i], max(0, c - (rlim - EPC - row0)) * ES);
+        }
+      }
+    }
+  }
+
+  // The chunk without its first n bytes, zeros behind.
+  static __device__ __forceinline__ i32x4 shifted(i32x4 v, int n) {
+    u64 lo = (u32)v[0] | (u64)(u32)v[1] << 32;
+    u64 hi = (u32)v[2] | (u64)(u32)v[3] << 32;
+    if (n >= 16) lo = hi = 0;
+    if (n >= 8) {
+      lo = hi;
+      hi = 0;
+      n -= 8;
+    }
+    if (n > 0 && n < 8) {
+      lo = lo >> 8 * n | hi << (64 - 8 * n);
+      hi >>= 8 * n;
+    }
+    return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+  }
+
+  __device__ __forceinline__ void load_slowly(i32x4 (&w)[IT], int tile,
+                                              int klim) const {
+    const E* s0 = (const E*)base;
     for (int i = 0; i < IT; ++i) {
       const int id = i * NT + (int)threadIdx.x;
       int n;  // elements of the chunk that exist
@@ -299,12 +360,14 @@ struct Side {
         s = s0 + (long)k * ld + row;
       }
       w[i] = i32x4{0, 0, 0, 0};
-      if (n >= EPC) {
-        __builtin_memcpy(&w[i], s, 16);  // global loads need no alignment
-      } else if (n > 0) {
-#pragma unroll
-        for (int j = 0; j < EPC; ++j)
-          if (j < n) w[i][j * ES / 4] |= (int)((u32)s[j] << (j * ES % 4 * 8));
+      for (int j = 0; j < EPC; ++j) {
+        if (j >= n) continue;
+        const int v = (int)((u32)s[j] << (j * ES % 4 * 8));
+        // selected, since a register cannot be indexed
+        if (j * ES / 4 == 0) w[i][0] |= v;
+        if (j * ES / 4 == 1) w[i][1] |= v;
+        if (j * ES / 4 == 2) w[i][2] |= v;
+        if (j * ES / 4 == 3) w[i][3] |= v;
       }
     }
   }
@@ -541,9 +604,9 @@ grouped_k(const GroupedArgs p) {
   if (tiles > 0) {
     SA sa;
     SB sb;
-    sa.init(p.a, p.lda, w.m0, w.mend, w.kbeg, FAST);
+    sa.init(p.a, p.lda, w.m0, w.mend, w.kbeg);
     sb.init((const char*)p.b + (WEIGHTS ? 0 : (long)w.g * p.gsb * ES), p.ldb,
-            w.n0, p.N, w.kbeg, FAST);
+            w.n0, p.N, w.kbeg);
     const int fast = FAST ? whole : 0;  // tiles that go straight to LDS
     int next = 0, to = 0;               // the next copy and its stage
     auto copy = [&]() {
@@ -561,8 +624,8 @@ grouped_k(const GroupedArgs p) {
     float rs = 0;
     auto load = [&](int tile) {
       if constexpr (SCALES) rs = scale[(long)tile * scale_step];
-      sa.load(ra, tile, w.kend);
-      sb.load(rb, tile, w.kend);
+      sa.load(ra, tile, w.kend, p.near_a);
+      sb.load(rb, tile, w.kend, p.near_b);
     };
     auto put = [&](int stage) {
       char* lds = smem + stage * STAGE;
@@ -727,12 +790,11 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     SA a0, a1;
     SB b0, b1;
     // a half past the end takes its row from inside
-    a0.init(p.a, p.lda, w.m0, w.mend, w.kbeg, true);
-    b0.init(b, p.ldb, w.n0, p.N, w.kbeg, true);
+    a0.init(p.a, p.lda, w.m0, w.mend, w.kbeg);
+    b0.init(b, p.ldb, w.n0, p.N, w.kbeg);
     a1.init(p.a, p.lda, w.m0 + 128 < w.mend ? w.m0 + 128 : w.m0, w.mend,
-            w.kbeg, true);
-    b1.init(b, p.ldb, w.n0 + 128 < p.N ? w.n0 + 128 : w.n0, p.N, w.kbeg,
-            true);
+            w.kbeg);
+    b1.init(b, p.ldb, w.n0 + 128 < p.N ? w.n0 + 128 : w.n0, p.N, w.kbeg);
 
     // Groups start at different K tiles: rows of many kilobytes lie a power of
     // two apart, and all XCDs, each in its own group, would read the same
@@ -804,13 +866,13 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       __syncthreads();
       typename SA::Regs r;
       typename SB::Regs s;
-      a0.load(r, whole, w.kend);
+      a0.load(r, whole, w.kend, true);
       SA::put(smem, r);
-      a1.load(r, whole, w.kend);
+      a1.load(r, whole, w.kend, true);
       SA::put(smem + HALF, r);
-      b0.load(s, whole, w.kend);
+      b0.load(s, whole, w.kend, true);
       SB::put(smem + 2 * HALF, s);
-      b1.load(s, whole, w.kend);
+      b1.load(s, whole, w.kend, true);
       SB::put(smem + 3 * HALF, s);
       load_scales(whole);
       __syncthreads();
