@@ -16,7 +16,7 @@ extern "C" {
 void launch_grouped_bf16(const GroupedArgs*, int, int, int, int, hipStream_t);
 void launch_grouped_f16(const GroupedArgs*, int, int, int, int, hipStream_t);
 void launch_grouped_f32(const GroupedArgs*, int, int, int, int, hipStream_t);
-void launch_grouped_fp8(const GroupedArgs*, int, int, int, hipStream_t);
+void launch_grouped_fp8(const GroupedArgs*, int, int, hipStream_t);
 void launch_grouped_join(const float*, void*, long, int, int, hipStream_t);
 void launch_fp8_quantize_row(const void*, int, long, long, long, void*,
                              float*, int, hipStream_t);
@@ -66,14 +66,15 @@ bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
          ld * t.element_size() < (1 << 24);
 }
 
-void set_offsets(GroupedArgs& p, const c10::optional<Tensor>& offs,
+void set_offsets(GroupedArgs& p, c10::optional<Tensor>& offs,
                  const Tensor& a, int64_t groups) {
   if (!offs.has_value()) {
     TORCH_CHECK(groups == 1, "several groups need offsets");
     return;
   }
+  offs = offs->contiguous();
   TORCH_CHECK(offs->device() == a.device() && offs->dim() == 1 &&
-                  offs->is_contiguous() && offs->numel() == groups + 1 &&
+                  offs->numel() == groups + 1 &&
                   (offs->scalar_type() == torch::kInt32 ||
                    offs->scalar_type() == torch::kInt64),
               "offsets must be groups + 1 integers on the operands' device");
@@ -90,8 +91,8 @@ int choose_tile(int64_t each, int64_t N, bool skinny) {
 }
 
 void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
-                 hipStream_t s, int aty = GT_FP8) {
-  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, aty, s);
+                 hipStream_t s) {
+  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, s);
   else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, fast, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, fast, s);
   else launch_grouped_f32(&p, tile, bk, 0, fast, s);
@@ -192,7 +193,7 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x);
 
 // c = a @ bt[group]^T of e4m3 operands: a [T, K] with scales [kb][T], or a
 // wider a without scales that is quantized by rows, bt [E, N, K] with scales
-// [E][kb][nb]. With `into` (f32, contiguous), the product is written there,
+// [E][kb][nb], or one matrix. With `into` (f32, contiguous), the product is written there,
 // or added where `accum` is set.
 Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
                         Tensor bsc, c10::optional<Tensor> offs,
@@ -200,14 +201,16 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
                         bool accum) {
   TORCH_CHECK(a.is_cuda() && bt.device() == a.device() &&
               bsc.device() == a.device(), "operands must be on one GPU");
+  if (bt.dim() == 2) {
+    bt = bt.unsqueeze(0);
+    bsc = bsc.unsqueeze(0);
+  }
   TORCH_CHECK(a.dim() == 2 && bt.dim() == 3 && a.size(1) == bt.size(2) &&
               bt.scalar_type() == torch::kFloat8_e4m3fn && bt.is_contiguous(),
               "operands do not match");
   const c10::hip::HIPGuard guard(a.device().index());
   const int64_t T = a.size(0), K = a.size(1), N = bt.size(1), E = bt.size(0);
   const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
-  int tile = choose_tile(E ? (T + E - 1) / E : 0, N, true);
-  int aty = GT_FP8;
   Tensor asc;
   if (a_scales.has_value()) {
     asc = *a_scales;
@@ -218,15 +221,7 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
                 asc.dim() == 2 && asc.size(0) == kb && asc.size(1) == T,
                 "scales of a must be float32 [ceil(K/128), rows]");
   } else {
-    TORCH_CHECK(K <= 1 || a.stride(1) == 1, "rows of a must be contiguous");
-    aty = type_of(a.scalar_type());
-    TORCH_CHECK(aty != GT_FP8, "e4m3 operands need scales");
-    // few 16-bit rows are quantized on the way into the product: the launch
-    // saved costs more than the conversion that every 16 columns repeat
-    if (tile != -1 || aty == GT_F32) {
-      std::tie(a, asc) = fp8_quantize_row(a);
-      aty = GT_FP8;
-    }
+    std::tie(a, asc) = fp8_quantize_row(a);
   }
   TORCH_CHECK(bsc.scalar_type() == torch::kFloat32 && bsc.is_contiguous() &&
               bsc.dim() == 3 && bsc.size(0) == E && bsc.size(1) == kb &&
@@ -253,9 +248,9 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   p.a = a.data_ptr();
   p.b = bt.data_ptr();
   p.c = c.data_ptr();
-  p.asc = asc.defined() ? asc.data_ptr<float>() : nullptr;
+  p.asc = asc.data_ptr<float>();
   p.bsc = bsc.data_ptr<float>();
-  p.lda = T > 1 ? a.stride(0) : 0;
+  p.lda = T > 1 ? K : 0;
   p.ldb = N > 1 ? K : 0;
   p.gsb = E > 1 ? N * K : 0;
   p.splits = 1;
@@ -265,7 +260,8 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   p.near_b = near_rows(bt, p.ldb, K);
   const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
                     aligned(bt, p.ldb, N) && aligned(bt, p.gsb, E);
-  launch_rows(p, GT_FP8, tile, true, fast, stream_of(a), aty);
+  launch_rows(p, GT_FP8, choose_tile((T + E - 1) / E, N, true), true, fast,
+              stream_of(a));
   return c;
 }
 

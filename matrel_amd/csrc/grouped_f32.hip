@@ -11,8 +11,8 @@ extern "C" void launch_grouped_f32(const GroupedArgs* p, int tile, int bk,
     if (!fast) grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, false>(*p, s);
     else grouped_go<TY, 128, 128, 2, 2, DM, false, false, true, true>(*p, s);
   } else if (tile < 0) {
-    if (tile == -1) grouped_skinny_go<TY, TY, 1>(*p, fast, s);
-    else grouped_skinny_go<TY, TY, 2>(*p, fast, s);
+    if (tile == -1) grouped_skinny_go<TY, 1>(*p, fast, s);
+    else grouped_skinny_go<TY, 2>(*p, fast, s);
   } else if (bk) {
     if (!fast) grouped_go<TY, 128, 128, 2, 2, 2, true, true, false, false>(*p, s);
     else if (tile >= 1) grouped_go<TY, 128, 128, 2, 2, DM, true, true, false, true>(*p, s);

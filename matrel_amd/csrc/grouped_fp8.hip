@@ -5,11 +5,9 @@
 #define DM 2
 
 extern "C" void launch_grouped_fp8(const GroupedArgs* p, int tile, int fast,
-                                   int aty, hipStream_t s) {
-  if (aty == GT_BF16) grouped_skinny_go<GT_FP8, GT_BF16, 1>(*p, fast, s);
-  else if (aty == GT_F16) grouped_skinny_go<GT_FP8, GT_F16, 1>(*p, fast, s);
-  else if (tile == -1) grouped_skinny_go<GT_FP8, GT_FP8, 1>(*p, fast, s);
-  else if (tile == -2) grouped_skinny_go<GT_FP8, GT_FP8, 2>(*p, fast, s);
+                                   hipStream_t s) {
+  if (tile == -1) grouped_skinny_go<GT_FP8, 1>(*p, fast, s);
+  else if (tile == -2) grouped_skinny_go<GT_FP8, 2>(*p, fast, s);
     else if (!fast) grouped_go<GT_FP8, 128, 128, 2, 2, 2, true, true, false, false>(*p, s);
   else if (tile == 2) grouped_big_go<GT_FP8, true, true, false>(*p, s);
   else if (tile == 1) grouped_go<GT_FP8, 128, 128, 2, 2, DM, true, true, false, true>(*p, s);

@@ -32,70 +32,20 @@ __device__ __forceinline__ i32x4 chunk_at(const typename Elt<TY>::T* row,
   return w;
 }
 
-template <int ATY> struct Values;  // 16 neighbouring values of a, in float32
-template <> struct Values<GT_FP8> {};  // never looked at
-template <> struct Values<GT_F32> {};
-template <int TY> struct Values16 {
-  i32x4 w[2];
-  __device__ __forceinline__ void load(const unsigned short* row, int k,
-                                       int klim) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) w[i] = chunk_at<TY>(row, k + 8 * i, klim);
-  }
-  __device__ __forceinline__ float get(int i) const {
-    const u32 d = (u32)w[i / 8][i % 8 / 2];
-    if constexpr (TY == GT_BF16)
-      return __uint_as_float(i % 2 ? d & 0xffff0000u : d << 16);
-    else
-      return (float)__builtin_bit_cast(
-          _Float16, (unsigned short)(i % 2 ? d >> 16 : d & 0xffffu));
-  }
-};
-template <> struct Values<GT_BF16> : Values16<GT_BF16> {};
-template <> struct Values<GT_F16> : Values16<GT_F16> {};
-
-// The quantization of quantize_row_k for the 128 values of a row that four
-// lanes hold, 32 each: their e4m3 and the row's scale.
-template <int ATY>
-__device__ __forceinline__ float quantize32(const Values<ATY> (&v)[2],
-                                            i32x4 (&y)[2]) {
-  u32 top = 0x0d800000u;  // 2^-100
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      top = max(top, __float_as_uint(v[h].get(j)) & 0x7fffffffu);
-  top = max(top, (u32)__shfl_xor((int)top, 16));
-  top = max(top, (u32)__shfl_xor((int)top, 32));
-  const float f = __uint_as_float(top), up = 448.0f / f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      int w = 0;
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(v[h].get(4 * d) * up,
-                                          v[h].get(4 * d + 1) * up, w, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(v[h].get(4 * d + 2) * up,
-                                          v[h].get(4 * d + 3) * up, w, true);
-      y[h][d] = w;
-    }
-  return f / 448.0f;
-}
-
-// 16 R rows of RB bytes a K tile, copied to LDS by one wave, 1 KB at a time.
-template <int RB, int ROWS> struct WaveSide {
-  static constexpr int N = RB * ROWS / 1024;
+// ROWS rows of a K tile, copied to LDS by one wave, 1 KB at a time.
+template <int ROWS> struct WaveSide {
+  static constexpr int N = ROWS / 8;
   u32 at[N];
   static __device__ __forceinline__ int swz(int c, int row) {
-    return RB == 128 ? c ^ (row >> 1 & 7) : c ^ (row & 15);
+    return c ^ (row >> 1 & 7);
   }
   // last: the last row that may be read, from the side's first one
   __device__ __forceinline__ void init(u32 ld_bytes, int last) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int id = i * 64 + lane, row = id / (RB / 16);
-      at[i] = (u32)min(row, last) * ld_bytes + swz(id % (RB / 16), row) * 16;
+      const int row = i * 8 + (lane >> 3);
+      at[i] = (u32)min(row, last) * ld_bytes + swz(lane & 7, row) * 16;
     }
   }
   __device__ __forceinline__ void copy(const char* tile, char* lds) const {
@@ -106,24 +56,19 @@ template <int RB, int ROWS> struct WaveSide {
   }
   static __device__ __forceinline__ i32x4 chunk(const char* lds, int row,
                                                 int c) {
-    return *(const i32x4*)(lds + row * RB + swz(c, row) * 16);
+    return *(const i32x4*)(lds + row * 128 + swz(c, row) * 16);
   }
 };
 
-// TY: the products' type. ATY: the type of a, which is TY, or, for TY fp8, a
-// wider type that is quantized here as quantize_row_k does it.
-template <int TY, int ATY, int MT, int NB, int W, bool FAST>
+template <int TY, int MT, int NB, int W, bool FAST>
 __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) {
   constexpr int ES = Elt<TY>::ES, EPC = 16 / ES, BKE = 128 / ES;
   constexpr int U = MT == 1 ? 4 : 2;  // K tiles at a time
-  constexpr bool QUANT = TY == GT_FP8 && ATY != GT_FP8;
   typedef typename Elt<TY>::T E;
-  typedef typename Elt<ATY>::T EA;
-  constexpr int RB = 128 * Elt<ATY>::ES / ES;  // bytes of a's rows a K tile
-  typedef WaveSide<128, 16> SX;
-  typedef WaveSide<RB, 16 * MT> SY;
+  typedef WaveSide<16> SX;
+  typedef WaveSide<16 * MT> SY;
   constexpr int SCALES = TY == GT_FP8 ? 256 : 0;
-  constexpr int STAGE = 2048 + 16 * MT * RB + SCALES;
+  constexpr int STAGE = 2048 + 16 * MT * 128 + SCALES;
   constexpr int D = 3;  // 4 and 5 stages a wave measured the same
   constexpr int OPS = SX::N + SY::N + (SCALES ? 1 : 0);  // copies a stage
   static_assert((D - 1) * OPS < 64, "counted by vmcnt");
@@ -149,12 +94,12 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
     for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0, 0, 0, 0};
 
   if (g < p.E) {
-    const EA* a[MT];
+    const E* a[MT];
     int row[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       row[i] = min(m0 + i * 16 + r, mend - 1);
-      a[i] = (const EA*)p.a + (long)row[i] * p.lda;
+      a[i] = (const E*)p.a + (long)row[i] * p.lda;
     }
     const int tiles = (p.K + BKE - 1) / BKE;
     const float* bsc = nullptr;
@@ -168,10 +113,10 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
       SX sx;
       SY sy;
       sx.init((u32)p.ldb * ES, p.N - 1 - n0);
-      sy.init((u32)p.lda * Elt<ATY>::ES, mend - 1 - m0);
+      sy.init((u32)p.lda * ES, mend - 1 - m0);
       const char* xb = (const char*)((const E*)p.b + (long)g * p.gsb +
                                      (long)n0 * p.ldb);
-      const char* yb = (const char*)((const EA*)p.a + (long)m0 * p.lda);
+      const char* yb = (const char*)((const E*)p.a + (long)m0 * p.lda);
       const long xstep = 16L * p.ldb * ES;
       char* ring = smem + wave * (D * STAGE);
       const int whole = p.K / BKE;
@@ -187,12 +132,12 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
         char* lds = ring + slot * STAGE;
         if constexpr (SCALES) {  // of the rows; behind them, of the columns
           const float* s = bsc + tile * nb;
-          if (!QUANT && lane < 16 * MT)
+          if (lane < 16 * MT)
             s = p.asc + tile * p.T + min(m0 + lane, mend - 1);
-          glds4(s, lds + 2048 + 16 * MT * RB + lane * 4);
+          glds4(s, lds + 2048 + 16 * MT * 128 + lane * 4);
         }
         sx.copy(cx + tile * 128, lds);
-        sy.copy(yb + tile * RB, lds + 2048);
+        sy.copy(yb + tile * 128, lds + 2048);
         if (++ci == mine) {
           ci = 0;
           // a block past the end reads the last one again
@@ -201,7 +146,7 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
       };
       auto product = [&](int slot, f32x4 (&acc)[MT]) {
         const char* lds = ring + slot * STAGE;
-        const float* sc = (const float*)(lds + 2048 + 16 * MT * RB);
+        const float* sc = (const float*)(lds + 2048 + 16 * MT * 128);
         i32x4 x[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) x[h] = SX::chunk(lds, r, h * 4 + q);
@@ -209,22 +154,10 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
         for (int i = 0; i < MT; ++i) {
           i32x4 y[2];
           float sa = 0;
-          if constexpr (QUANT) {
-            Values<ATY> v[2];
-            constexpr int C = RB / 128;  // chunks of 16 values
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int c = 0; c < C; ++c)
-                v[h].w[c] = SY::chunk(lds + 2048, i * 16 + r,
-                                      (h * 4 + q) * C + c);
-            sa = quantize32<ATY>(v, y);
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              y[h] = SY::chunk(lds + 2048, i * 16 + r, h * 4 + q);
-            if constexpr (TY == GT_FP8) sa = sc[i * 16 + r];
-          }
+          for (int h = 0; h < 2; ++h)
+            y[h] = SY::chunk(lds + 2048, i * 16 + r, h * 4 + q);
+          if constexpr (TY == GT_FP8) sa = sc[i * 16 + r];
           if constexpr (TY == GT_FP8) {
             const float s = sa * sc[16 * MT];
             const f32x4 d = mma_fp8(join8(x[0], x[1]), join8(y[0], y[1]),
@@ -265,7 +198,6 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
       const E* b = (const E*)p.b + (long)g * p.gsb +
                    (long)min(n0 + nbk * 16 + r, p.N - 1) * p.ldb;
       i32x4 x[U][2], y[U][MT][2];
-      Values<ATY> v[QUANT ? U : 1][QUANT ? MT : 1][2];
       float sa[U][MT], sb[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -278,13 +210,9 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if constexpr (QUANT)
-              v[u][i][h].load(a[i], k + (h * 4 + q) * EPC, p.K);
-            else
-              y[u][i][h] = chunk_at<ATY>(a[i], k + (h * 4 + q) * EPC, p.K);
-          }
-          if constexpr (TY == GT_FP8 && !QUANT)
+          for (int h = 0; h < 2; ++h)
+            y[u][i][h] = chunk_at<TY>(a[i], k + (h * 4 + q) * EPC, p.K);
+          if constexpr (TY == GT_FP8)
             sa[u][i] = tile < tiles ? p.asc[(long)tile * p.T + row[i]] : 0;
         }
       }
@@ -292,9 +220,6 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          if constexpr (QUANT) {
-            sa[u][i] = quantize32<ATY>(v[u][i], y[u][i]);
-          }
           if constexpr (TY == GT_FP8) {
             const f32x4 d = mma_fp8(join8(x[u][0], x[u][1]),
                                     join8(y[u][i][0], y[u][i][1]),
@@ -337,13 +262,13 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
   }
 }
 
-template <int TY, int ATY, int MT, int NB>
+template <int TY, int MT, int NB>
 static void grouped_skinny_nb(const GroupedArgs& p, bool fast, bool eight,
                               hipStream_t s) {
   const long wgs =
       (p.T / (16 * MT) + p.E + 2L) * ((p.N + 16 * NB - 1) / (16 * NB));
 #define GO(W, FAST)                                                         \
-  hipLaunchKernelGGL((grouped_skinny_k<TY, ATY, MT, NB, W, FAST>),          \
+  hipLaunchKernelGGL((grouped_skinny_k<TY, MT, NB, W, FAST>),          \
                      dim3((unsigned)wgs), dim3(64 * W), 0, s, p)
   if (fast && eight) GO(8, true);
   else if (fast) GO(4, true);
@@ -358,17 +283,17 @@ static void grouped_skinny_nb(const GroupedArgs& p, bool fast, bool eight,
 // blocks: 73 / 52 / 61 us; one row, 4096 x 4096 (256): 8.5 / 11.1 / 15.3 us;
 // fp8, 64 rows in 32 groups of 4096 x 2048 (9216): 43 / 34 / 31 us. With few
 // blocks and a long sum, eight waves share it instead of four.
-template <int TY, int ATY, int MT>
+template <int TY, int MT>
 static void grouped_skinny_go(const GroupedArgs& p, bool fast,
                               hipStream_t s) {
   const long blocks =
       ((long)p.T / (16 * MT) + std::min(p.E, p.T)) * ((p.N + 15) / 16);
   const int tiles = (p.K + 128 / Elt<TY>::ES - 1) / (128 / Elt<TY>::ES);
   if (blocks >= 8192)
-    grouped_skinny_nb<TY, ATY, MT, 4>(p, fast, false, s);
+    grouped_skinny_nb<TY, MT, 4>(p, fast, false, s);
   else if (blocks >= 512)
-    grouped_skinny_nb<TY, ATY, MT, 2>(p, fast, false, s);
+    grouped_skinny_nb<TY, MT, 2>(p, fast, false, s);
   else
-    grouped_skinny_nb<TY, ATY, MT, 1>(p, fast, tiles >= 64 && blocks <= 256,
+    grouped_skinny_nb<TY, MT, 1>(p, fast, tiles >= 64 && blocks <= 256,
                                       s);
 }

@@ -22,7 +22,7 @@ import torch
 
 from .backend import require_ext, use_hip
 from .grouped import (check_capture, check_offsets, check_out_dtype,
-                      rows_contiguous, rows_product, weights_product)
+                      needs_grad, rows_contiguous, rows_product, weights_product)
 
 BLOCK = 128
 _MAX = 448.0
@@ -65,6 +65,13 @@ class Fp8Blocks:
             raise ValueError("data and scale must be on one device")
         if not (d.is_contiguous() and s.is_contiguous()):
             raise ValueError("data and scale must be contiguous")
+
+    @classmethod
+    def _made(cls, data, scale, kind) -> "Fp8Blocks":
+        """Blocks that were made here and need no checks."""
+        q = object.__new__(cls)
+        q.data, q.scale, q.kind = data, scale, kind
+        return q
 
     @property
     def shape(self) -> torch.Size:
@@ -137,10 +144,11 @@ def quantize_fp8(x: torch.Tensor, kind: str = "row") -> Fp8Blocks:
     if kind == "tile":
         q, s, _, _ = e.fp8_quantize_tile(x if x.dim() == 3 else x[None],
                                          False)
-        return Fp8Blocks(q, s, kind) if x.dim() == 3 else \
-            Fp8Blocks(q[0], s[0], kind)
+        return Fp8Blocks._made(q, s, kind) if x.dim() == 3 else \
+            Fp8Blocks._made(q[0], s[0], kind)
     if x.dim() == 2:
-        return Fp8Blocks(*e.fp8_quantize_row(x), kind)
+        q, s = e.fp8_quantize_row(x)
+        return Fp8Blocks._made(q, s, kind)
     n, r, c = x.shape
     q, s = e.fp8_quantize_row(x.reshape(n * r, c))
     s = s.reshape(s.shape[0], n, r).transpose(0, 1).contiguous()
@@ -149,22 +157,18 @@ def quantize_fp8(x: torch.Tensor, kind: str = "row") -> Fp8Blocks:
 
 def _product(a, bt: Fp8Blocks, offsets, out_dtype):
     """a @ bt[group]^T; a: blocks, or values to be quantized; bt [groups, n,
-    k]."""
+    k] or [n, k]."""
     blocks = isinstance(a, Fp8Blocks)
     if not use_hip(bt.data):
         q = a if blocks else _cpu_quantize(a, "row")
-        return rows_product(q.dequantize(), bt.dequantize().transpose(1, 2),
+        w = bt.dequantize()
+        return rows_product(q.dequantize(),
+                            (w if w.dim() == 3 else w[None]).transpose(1, 2),
                             offsets, out_dtype)
     return require_ext().grouped_rows_fp8(
         a.data if blocks else rows_contiguous(a),
-        a.scale if blocks else None, bt.data, bt.scale,
-        None if offsets is None else offsets.contiguous(), out_dtype, None,
-        False)
-
-
-def _stack(q: Fp8Blocks) -> Fp8Blocks:
-    return q if q.data.dim() == 3 else \
-        Fp8Blocks(q.data[None], q.scale[None], q.kind)
+        a.scale if blocks else None, bt.data, bt.scale, offsets, out_dtype,
+        None, False)
 
 
 def _quantize_both(w: torch.Tensor):
@@ -173,7 +177,7 @@ def _quantize_both(w: torch.Tensor):
         q = _cpu_quantize(w, "tile")
         return q, q.transpose()
     q, s, qt, st = require_ext().fp8_quantize_tile(rows_contiguous(w), True)
-    return Fp8Blocks(q, s, "tile"), Fp8Blocks(qt, st, "tile")
+    return Fp8Blocks._made(q, s, "tile"), Fp8Blocks._made(qt, st, "tile")
 
 
 class _Fp8Matmul(torch.autograd.Function):
@@ -182,7 +186,7 @@ class _Fp8Matmul(torch.autograd.Function):
         w3 = None if w is None else (w if w.dim() == 3 else w[None])
         turned = None
         if w is None:
-            q = _stack(frozen)
+            q = frozen
         elif ctx.needs_input_grad[0]:
             q, turned = _quantize_both(w3)
         else:
@@ -256,11 +260,15 @@ def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
             if bt.requires_grad and torch.is_grad_enabled():
                 raise ValueError("the gradient of bt needs a as a tensor")
             bt = quantize_fp8(bt, "tile")
-        return _product(a, _stack(bt), offsets, out_dtype)
+        return _product(a, bt, offsets, out_dtype)
     if isinstance(bt, torch.Tensor):
         if bt.dtype != a.dtype:
             raise TypeError(f"a is {a.dtype}, bt {bt.dtype}")
-        check_capture(a, bt)
-        return _Fp8Matmul.apply(a, bt, None, offsets, out_dtype)
-    check_capture(a)
-    return _Fp8Matmul.apply(a, None, bt, offsets, out_dtype)
+        if needs_grad(a, bt):
+            check_capture(a, bt)
+            return _Fp8Matmul.apply(a, bt, None, offsets, out_dtype)
+        bt = quantize_fp8(bt, "tile")
+    elif needs_grad(a):
+        check_capture(a)
+        return _Fp8Matmul.apply(a, None, bt, offsets, out_dtype)
+    return _product(a, bt, offsets, out_dtype)

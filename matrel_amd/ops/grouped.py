@@ -53,18 +53,20 @@ def check_out_dtype(out_dtype: Optional[torch.dtype],
     return out_dtype
 
 
+def needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
 def check_capture(*leaves) -> None:
     """Autograd runs a leaf's accumulation on the stream of the graph that
     met it first. A backward pass captured while such an outside graph lives
     would make the capture wait for that stream, which ends the process: it
     is refused here, before anything is recorded."""
-    if not torch.cuda.is_available() \
-            or not torch.cuda.is_current_stream_capturing() \
-            or not torch.is_grad_enabled():
+    if not leaves[0].is_cuda \
+            or not torch.cuda.is_current_stream_capturing():
         return
     for t in leaves:
-        if isinstance(t, torch.Tensor) and t.is_cuda \
-                and require_ext().has_grad_accumulator(t):
+        if require_ext().has_grad_accumulator(t):
             raise RuntimeError(
                 "an autograd graph built outside of this capture still "
                 "holds an operand: free it (its loss and outputs) before "
@@ -102,7 +104,6 @@ def rows_product(a, b, offsets, out_dtype):
     """c[t] = a[t] @ b[group of t]; offsets None: one group of all rows."""
     if not use_hip(a):
         return _cpu_rows(a, b, offsets, out_dtype)
-    offsets = None if offsets is None else offsets.contiguous()
     return require_ext().grouped_rows(
         rows_contiguous(a), _matrix_contiguous(b), offsets, out_dtype)
 
@@ -111,7 +112,6 @@ def weights_product(a, b, offsets, groups, out_dtype):
     """c[g] = a_g^T @ b_g over the rows of each group."""
     if not use_hip(a):
         return _cpu_weights(a, b, offsets, groups, out_dtype)
-    offsets = None if offsets is None else offsets.contiguous()
     return require_ext().grouped_weights(
         rows_contiguous(a), rows_contiguous(b), offsets, groups, out_dtype)
 
@@ -194,5 +194,7 @@ def grouped_matmul(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     in a and b."""
     _check(a, b, offsets)
     out_dtype = check_out_dtype(out_dtype, a.dtype)
+    if not needs_grad(a, b):
+        return rows_product(a, b, offsets, out_dtype)
     check_capture(a, b)
     return _GroupedMatmul.apply(a, b, offsets, out_dtype)
