@@ -7,7 +7,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
-#include <limits>
+#include <algorithm>
 #include <tuple>
 
 #include "grouped_args.h"
@@ -59,11 +59,11 @@ bool aligned(const Tensor& t, int64_t ld, int64_t count) {
          (count <= 1 || ld * es % 16 == 0);
 }
 
-// A row of `len` elements holds 16 bytes, and a tile's 256 rows lie within 32
+// A row of `len` elements holds 16 bytes, and a tile's 256 rows lie within 31
 // bits of its first one.
 bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
   return len * t.element_size() >= 16 &&
-         ld * t.element_size() < (1 << 24);
+         ld * t.element_size() < (1 << 23);
 }
 
 void set_offsets(GroupedArgs& p, c10::optional<Tensor>& offs,
@@ -82,12 +82,71 @@ void set_offsets(GroupedArgs& p, c10::optional<Tensor>& offs,
   p.off64 = offs->scalar_type() == torch::kInt64;
 }
 
-// The tile for a product of `each` rows a group on average: 2: 256 x 256,
-// 1: 128 x 128, 0: 32 x 128, -1, -2: 16 columns of 16, 32 rows.
-int choose_tile(int64_t each, int64_t N, bool skinny) {
-  if (skinny && each <= 32) return each <= 16 ? -1 : -2;
-  if (each > 128 && N > 128) return 2;
-  return each > 32 ? 1 : 0;
+struct Plan {
+  int tile, splits;
+};
+
+// The largest tile whose number fills the chip (codes: grouped_launch.h), and
+// into how many parts long sums are split where even small tiles do not.
+// count(bm, bn): tiles of a size. Measured, us (64 x 64 / 128 x 128 / 256 x
+// 256; the rule counts 128 x 128 tiles):
+//   bf16 4096 rows, 12 groups, 1024 x 1000 (352): 34 / 26 / 31
+//   bf16 300 rows, 4 groups, 2048 x 1024 (96): 9 / 17 / 25
+//   fp8 5003 rows, 24 groups, 1536 x 2560 (756): 66 / 68 / 46
+//   f32 4096 rows, 12 groups, 1024 x 1000 (352): 106 / 138 / -
+//   fp16 unaligned, 3001 rows, 10 groups, 1111 x 777, d_b (630): 36 / 50 / -
+int choose_splits(int64_t tiles, int64_t k_tiles) {
+  // the join is a launch and a pass over the parts: not for short sums
+  if (tiles >= 192 || k_tiles < 16) return 1;
+  return (int)std::min<int64_t>({k_tiles / 4, (383 + tiles) / tiles, 16});
+}
+
+template <class F>
+Plan choose(int ty, bool fast, int64_t k_tiles, F count) {
+  Plan p = {1, 1};
+  const int64_t middle = count(128, 128);
+  if (fast && ty != GT_F32 && count(256, 256) >= 200) p.tile = 3;
+  else if (middle >= (fast && ty != GT_F32 ? 250 : 1024)) p.tile = 2;
+  if (p.tile == 1) p.splits = choose_splits(count(64, 64), k_tiles);
+  return p;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles of the rows of E groups, each of which can end inside a tile.
+int64_t row_tiles(int64_t T, int64_t E, int64_t bm) {
+  return E == 1 ? ceil_div(T, bm) : T / bm + std::min(E, T);
+}
+
+Plan choose_rows(int ty, bool bk, bool fast, int64_t T, int64_t E, int64_t K,
+                 int64_t N) {
+  const int64_t each = ceil_div(T, E);
+  const int64_t k_tiles = ceil_div(K, ty == GT_FP8 ? 128
+                                      : ty == GT_F32 ? 32 : 64);
+  if (bk && each <= 32) return {each <= 16 ? -1 : -2, 1};
+  if (fast && each <= 32)
+    return {0, choose_splits(row_tiles(T, E, 32) * ceil_div(N, 128), k_tiles)};
+  return choose(ty, fast, k_tiles, [&](int64_t bm, int64_t bn) {
+    return row_tiles(T, E, bm) * ceil_div(N, bn);
+  });
+}
+
+// Where the kernel writes: c, or partial sums that finish() joins.
+Tensor begin(GroupedArgs& p, Tensor& c, int splits) {
+  Tensor part;
+  p.splits = splits;
+  if (splits > 1) {
+    part = torch::empty({splits, c.numel()},
+                        c.options().dtype(torch::kFloat32));
+    p.part = part.data_ptr<float>();
+  }
+  return part;
+}
+
+void finish(const GroupedArgs& p, Tensor& c, hipStream_t s) {
+  if (p.splits > 1)
+    launch_grouped_join(p.part, p.c, c.numel(), p.splits, p.out, s);
+  check_launch();
 }
 
 void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
@@ -96,7 +155,6 @@ void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
   else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, fast, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, fast, s);
   else launch_grouped_f32(&p, tile, bk, 0, fast, s);
-  check_launch();
 }
 
 // c[t, :] = a[t, :] @ b[group of t], zeros for rows of no group.
@@ -131,15 +189,17 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.lda = T > 1 ? a.stride(0) : 0;
   p.ldb = bk ? (N > 1 ? b.stride(2) : 0) : b.stride(1);
   p.gsb = E > 1 ? b.stride(0) : 0;
-  p.splits = 1;
   p.out = type_of(out);
   p.near_a = near_rows(a, p.lda, K);
   p.near_b = near_rows(b, p.ldb, bk ? K : N);
   const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
                     aligned(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
                     (bk || N % epc == 0);
-  const int tile = choose_tile((T + E - 1) / E, N, bk);
-  launch_rows(p, ty, tile, bk, fast, stream_of(a));
+  const Plan plan = choose_rows(ty, bk, fast, T, E, K, N);
+  const hipStream_t s = stream_of(a);
+  const Tensor part = begin(p, c, plan.splits);
+  launch_rows(p, ty, plan.tile, bk, fast, s);
+  finish(p, c, s);
   return c;
 }
 
@@ -173,19 +233,23 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.c = c.data_ptr();
   p.lda = T > 1 ? a.stride(0) : 0;
   p.ldb = T > 1 ? b.stride(0) : 0;
-  p.splits = 1;
   p.out = type_of(out);
   p.near_a = near_rows(a, p.lda, M);
   p.near_b = near_rows(b, p.ldb, N);
   const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
                     aligned(b, p.ldb, T) &&
                     M % epc == 0 && N % epc == 0;
-  const int tile = choose_tile(M, N, false);
+  const int64_t k_tiles = T / E / (ty == GT_F32 ? 32 : 64);
+  const Plan plan = choose(ty, fast, k_tiles, [&](int64_t bm, int64_t bn) {
+    return E * ceil_div(M, bm) * ceil_div(N, bn);
+  });
+  const int tile = plan.tile;
   const hipStream_t s = stream_of(a);
+  const Tensor part = begin(p, c, plan.splits);
   if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, fast, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, fast, s);
   else launch_grouped_f32(&p, tile, 0, 1, fast, s);
-  check_launch();
+  finish(p, c, s);
   return c;
 }
 
@@ -253,15 +317,17 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   p.lda = T > 1 ? K : 0;
   p.ldb = N > 1 ? K : 0;
   p.gsb = E > 1 ? N * K : 0;
-  p.splits = 1;
   p.out = type_of(c.scalar_type());
   p.accum = accum;
   p.near_a = near_rows(a, p.lda, K);
   p.near_b = near_rows(bt, p.ldb, K);
   const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
                     aligned(bt, p.ldb, N) && aligned(bt, p.gsb, E);
-  launch_rows(p, GT_FP8, choose_tile((T + E - 1) / E, N, true), true, fast,
-              stream_of(a));
+  const Plan plan = choose_rows(GT_FP8, true, fast, T, E, K, N);
+  const hipStream_t s = stream_of(a);
+  const Tensor part = begin(p, c, accum ? 1 : plan.splits);
+  launch_rows(p, GT_FP8, plan.tile, true, fast, s);
+  finish(p, c, s);
   return c;
 }
 

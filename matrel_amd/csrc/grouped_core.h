@@ -193,6 +193,27 @@ __device__ __forceinline__ bool find_row_tile(const GroupedArgs& p, int ntn,
   return false;
 }
 
+// The group with the n-th longest range and that range, for up to 64 groups:
+// long sums begin first and short ones fill what they leave (f32, 8192 rows
+// in 4 uneven groups, 2048 x 2048: 1061 -> 503 us). It takes a microsecond,
+// which sums over few rows do not repay.
+__device__ __forceinline__ void by_length(const GroupedArgs& p, int n,
+                                          int* g, int* lo, int* hi) {
+  const int lane = threadIdx.x & 63;
+  const int a = bound_at(p, lane + 1), b = max(a, bound_at(p, lane + 2));
+  const int len = lane < p.E ? b - a : -1;
+  int rank = 0;
+  for (int j = 0; j < p.E; ++j) {
+    const int other = __builtin_amdgcn_readlane(len, j);
+    rank += other > len || (other == len && j < lane);
+  }
+  const int at =
+      __ffsll((unsigned long long)__ballot(rank == n && lane < p.E)) - 1;
+  *g = at;
+  *lo = __builtin_amdgcn_readlane(a, at);
+  *hi = __builtin_amdgcn_readlane(b, at);
+}
+
 // ---- operands --------------------------------------------------------------
 
 // An operand's tile of R rows x 128 bytes of k in LDS, filled by NT threads.
@@ -207,7 +228,7 @@ struct Side {
   static constexpr int CPR = R * ES / 16;      // R side: chunks of one k
   static_assert(R * 8 % NT == 0, "whole chunks for every thread");
 
-  u32 at[IT];        // this thread's chunks of a tile, bytes from `base`
+  int at[IT];        // this thread's chunks of a tile, bytes from `base`
   const char* base;  // the operand's first row (R side: column) and k
   long ld;
   int row0, rlim, k0;
@@ -215,9 +236,13 @@ struct Side {
   // R side, swizzled chunk c at k <-> the chunk as it lies in memory.
   // 16 bits: the 16 lanes of a transposing read take 32 bytes at each of 4 k,
   // and 4 such groups run at once (k = 8g + j): 32-byte slots are permuted by
-  // j and g's low bit. f32: 64-byte slots by k / 4.
+  // j and g's low bit; of 64 rows two k share the 256 bytes of all banks, and
+  // there are 4 slots. f32: 64-byte slots by k / 4.
+  static_assert(KROWS || R >= 64, "R side: at least 4 slots");
   static __device__ __forceinline__ int swz(int c, int k) {
-    if constexpr (ES == 2) {
+    if constexpr (ES == 2 && R == 64) {
+      return c ^ ((k >> 1 & 1) | (k >> 3 & 1) << 1) << 1;
+    } else if constexpr (ES == 2) {
       return c ^ (((k & 3) | (k >> 3 & 1) << 2) << 1);
     } else {
       return c ^ (k >> 2 & 3) << 2;
@@ -240,11 +265,11 @@ struct Side {
       const int id = i * NT + (int)threadIdx.x;
       if constexpr (KROWS) {
         const int row = id >> 3, c = (id & 7) ^ (row >> 1 & 7);
-        at[i] = (u32)min(row, rlim - 1 - row0) * (u32)ld * ES + c * 16;
+        at[i] = min(row, rlim - 1 - row0) * (int)ld * ES + c * 16;
       } else {
         const int k = id / CPR, c = swz(id % CPR, k);
-        at[i] = (u32)k * (u32)ld * ES +
-                (u32)(min(c * EPC, rlim - EPC - row0) * ES);
+        // below zero where the last tile is narrower than a chunk
+        at[i] = k * (int)ld * ES + min(c * EPC, rlim - EPC - row0) * ES;
       }
     }
   }
@@ -279,7 +304,9 @@ struct Side {
   // Any tile, any alignment: through registers, zeros for k >= klim.
   // Loads stay free of branches (one inside would wait for the one before):
   // a chunk that ends early is read from further in front and shifted.
-  // near: a row has at least a chunk, and offsets fit 32 bits.
+  // near: a row has at least a chunk, and offsets fit 31 bits.
+  // PARTS: the last chunk of an R side's rows may be a part of one.
+  template <bool PARTS>
   __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile, int klim,
                                        bool near) const {
     if (!near) {
@@ -293,27 +320,27 @@ struct Side {
       for (int i = 0; i < IT; ++i)  // global loads need no alignment
         __builtin_memcpy(&w[i], s + at[i], 16);
     } else {
-      long back[IT];
+      int back[IT];
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int id = i * NT + (int)threadIdx.x;
         if constexpr (KROWS)
           back[i] = max(0, (((id & 7) ^ (id >> 4 & 7)) + 1) * EPC - k1) * ES;
         else
-          back[i] = max(0, id / CPR + 1 - k1) * ld * ES;
+          back[i] = max(0, id / CPR + 1 - k1) * (int)ld * ES;
       }
 #pragma unroll
       for (int i = 0; i < IT; ++i)
-        __builtin_memcpy(&w[i], s + at[i] - back[i], 16);
+        __builtin_memcpy(&w[i], s + ((long)at[i] - back[i]), 16);
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        if constexpr (KROWS) w[i] = shifted(w[i], (int)back[i]);
+        if constexpr (KROWS) w[i] = shifted(w[i], back[i]);
         else if ((i * NT + (int)threadIdx.x) / CPR >= k1)
           w[i] = i32x4{0, 0, 0, 0};
       }
     }
-    if constexpr (!KROWS) {
-      if (row0 + R > rlim) {  // the last chunk of rows may be a part
+    if constexpr (!KROWS && PARTS) {
+      if (row0 + R > rlim) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
           const int id = i * NT + (int)threadIdx.x;
@@ -432,13 +459,17 @@ __device__ __forceinline__ bool locate(const GroupedArgs& p, Work* w) {
     const int ntm = (p.M + BM - 1) / BM, per = ntm * ntn;
     w->g = blockIdx.x / per;
     const int rem = (int)xcd_swizzle(blockIdx.x - w->g * per, per);
+    if (p.E > 1 && p.E <= 64 && p.T >= 256 * p.E) {
+      by_length(p, w->g, &w->g, &w->kbeg, &w->kend);
+    } else {
+      w->kbeg = bound_at(p, w->g + 1);
+      w->kend = max(w->kbeg, bound_at(p, w->g + 2));
+    }
     const int band = rem / (8 * ntn), r = rem - band * 8 * ntn;
     const int wide = min(8, ntm - band * 8);
     w->m0 = (band * 8 + r % wide) * BM;
     w->n0 = r / wide * BN;
     w->mend = p.M;
-    w->kbeg = bound_at(p, w->g + 1);
-    w->kend = max(w->kbeg, bound_at(p, w->g + 2));
   } else {
     RowTile t;
     if (!find_row_tile<BM>(p, ntn, &t)) return false;
@@ -516,7 +547,7 @@ template <bool WEIGHTS> struct Results {
 // LDS behind them.
 template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
           bool WEIGHTS, bool FAST>
-__global__ void __launch_bounds__(64 * WM * WN)
+__global__ void __launch_bounds__(64 * WM * WN, 2)  // waves a SIMD
 grouped_k(const GroupedArgs p) {
   constexpr int NT = 64 * WM * WN;
   constexpr int ES = Elt<TY>::ES, BKE = 128 / ES;
@@ -624,8 +655,8 @@ grouped_k(const GroupedArgs p) {
     float rs = 0;
     auto load = [&](int tile) {
       if constexpr (SCALES) rs = scale[(long)tile * scale_step];
-      sa.load(ra, tile, w.kend, p.near_a);
-      sb.load(rb, tile, w.kend, p.near_b);
+      sa.template load<!FAST>(ra, tile, w.kend, p.near_a);
+      sb.template load<!FAST>(rb, tile, w.kend, p.near_b);
     };
     auto put = [&](int stage) {
       char* lds = smem + stage * STAGE;
@@ -866,13 +897,13 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       __syncthreads();
       typename SA::Regs r;
       typename SB::Regs s;
-      a0.load(r, whole, w.kend, true);
+      a0.template load<false>(r, whole, w.kend, true);
       SA::put(smem, r);
-      a1.load(r, whole, w.kend, true);
+      a1.template load<false>(r, whole, w.kend, true);
       SA::put(smem + HALF, r);
-      b0.load(s, whole, w.kend, true);
+      b0.template load<false>(s, whole, w.kend, true);
       SB::put(smem + 2 * HALF, s);
-      b1.load(s, whole, w.kend, true);
+      b1.template load<false>(s, whole, w.kend, true);
       SB::put(smem + 3 * HALF, s);
       load_scales(whole);
       __syncthreads();

@@ -1,6 +1,7 @@
 // Tile choice and launch of grouped_k, one translation unit a type.
 #pragma once
 #include "grouped_core.h"
+#include "grouped_skinny.h"
 
 template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
           bool WEIGHTS, bool FAST>
@@ -24,4 +25,45 @@ static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
   auto k = grouped_big_k<TY, AK, BK, WEIGHTS>;
   hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
                      dim3(512), 2 * 4 * 128 * 128, s, p);
+}
+
+// Tile codes, as choose_tile (ext_grouped.cpp) picks them.
+//   -1, -2: 16, 32 rows, columns by 16 (b with k along its rows)
+//   0: 32 x 128   1: 64 x 64   2: 128 x 128   3: 256 x 256 (not f32)
+// Stages are as many as let two workgroups share the LDS of a CU.
+template <int TY, bool BK>
+static void launch_rows_tile(const GroupedArgs& p, int tile, bool fast,
+                             hipStream_t s) {
+  if constexpr (BK) {
+    if (tile == -1) return grouped_skinny_go<TY, 1>(p, fast, s);
+    if (tile == -2) return grouped_skinny_go<TY, 2>(p, fast, s);
+  }
+  if (!fast) {
+    if (tile == 2)
+      return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, false>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 2, true, BK, false, false>(p, s);
+  }
+  if constexpr (TY != GT_F32)
+    if (tile == 3) return grouped_big_go<TY, true, BK, false>(p, s);
+  if (tile >= 2)
+    return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, true>(p, s);
+  if (tile == 1)
+    return grouped_go<TY, 64, 64, 2, 2, 4, true, BK, false, true>(p, s);
+  if constexpr (!BK)  // with k along b's rows, -1 and -2 take few rows
+    grouped_go<TY, 32, 128, 1, 4, 3, true, BK, false, true>(p, s);
+}
+
+template <int TY>
+static void launch_weights_tile(const GroupedArgs& p, int tile, bool fast,
+                                hipStream_t s) {
+  if (!fast) {
+    if (tile >= 2)
+      return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, false>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 2, false, false, true, false>(p, s);
+  }
+  if constexpr (TY != GT_F32)
+    if (tile == 3) return grouped_big_go<TY, false, false, true>(p, s);
+  if (tile >= 2)
+    return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, true>(p, s);
+  grouped_go<TY, 64, 64, 2, 2, 4, false, false, true, true>(p, s);
 }

@@ -77,6 +77,8 @@ SHAPES = [
     ([300, 290], 264, 520),
     ([7, 200, 0, 61], 77, 111),
     ([17, 3], 1000, 9),
+    ([70, 2, 131], 67, 131),  # last tiles narrower than 16 bytes
+    ([50], 3, 5),  # rows shorter than 16 bytes
     ([0, 0], 16, 16),
 ]
 
