@@ -19,9 +19,9 @@ void launch_grouped_f32(const GroupedArgs*, int, int, int, int, hipStream_t);
 void launch_grouped_fp8(const GroupedArgs*, int, int, hipStream_t);
 void launch_grouped_join(const float*, void*, long, int, int, hipStream_t);
 void launch_fp8_quantize_row(const void*, int, long, long, long, void*,
-                             float*, int, hipStream_t);
+                             float*, hipStream_t);
 void launch_fp8_quantize_tile(const void*, int, long, long, long, long, long,
-                              void*, void*, float*, float*, int, hipStream_t);
+                              void*, void*, float*, float*, hipStream_t);
 }
 
 namespace {
@@ -61,6 +61,7 @@ bool aligned(const Tensor& t, int64_t ld, int64_t count) {
 
 // A row of `len` elements holds 16 bytes, and a tile's 256 rows lie within 31
 // bits of its first one.
+// Neither alignment (path 1) nor that (path 2) is asked of the operands.
 bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
   return len * t.element_size() >= 16 &&
          ld * t.element_size() < (1 << 23);
@@ -149,12 +150,12 @@ void finish(const GroupedArgs& p, Tensor& c, hipStream_t s) {
   check_launch();
 }
 
-void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, bool fast,
+void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, int path,
                  hipStream_t s) {
-  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, fast, s);
-  else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, fast, s);
-  else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, fast, s);
-  else launch_grouped_f32(&p, tile, bk, 0, fast, s);
+  if (ty == GT_FP8) launch_grouped_fp8(&p, tile, path, s);
+  else if (ty == GT_BF16) launch_grouped_bf16(&p, tile, bk, 0, path, s);
+  else if (ty == GT_F16) launch_grouped_f16(&p, tile, bk, 0, path, s);
+  else launch_grouped_f32(&p, tile, bk, 0, path, s);
 }
 
 // c[t, :] = a[t, :] @ b[group of t], zeros for rows of no group.
@@ -190,15 +191,15 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.ldb = bk ? (N > 1 ? b.stride(2) : 0) : b.stride(1);
   p.gsb = E > 1 ? b.stride(0) : 0;
   p.out = type_of(out);
-  p.near_a = near_rows(a, p.lda, K);
-  p.near_b = near_rows(b, p.ldb, bk ? K : N);
-  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
-                    aligned(b, p.ldb, bk ? N : K) && aligned(b, p.gsb, E) &&
-                    (bk || N % epc == 0);
-  const Plan plan = choose_rows(ty, bk, fast, T, E, K, N);
+  const int path = !near_rows(a, p.lda, K) ||
+                           !near_rows(b, p.ldb, bk ? K : N) ? 2
+                   : aligned(a, p.lda, T) && aligned(b, p.ldb, bk ? N : K) &&
+                           aligned(b, p.gsb, E) && (bk || N % epc == 0) ? 0
+                   : 1;
+  const Plan plan = choose_rows(ty, bk, path == 0, T, E, K, N);
   const hipStream_t s = stream_of(a);
   const Tensor part = begin(p, c, plan.splits);
-  launch_rows(p, ty, plan.tile, bk, fast, s);
+  launch_rows(p, ty, plan.tile, bk, path, s);
   finish(p, c, s);
   return c;
 }
@@ -234,21 +235,20 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   p.lda = T > 1 ? a.stride(0) : 0;
   p.ldb = T > 1 ? b.stride(0) : 0;
   p.out = type_of(out);
-  p.near_a = near_rows(a, p.lda, M);
-  p.near_b = near_rows(b, p.ldb, N);
-  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
-                    aligned(b, p.ldb, T) &&
-                    M % epc == 0 && N % epc == 0;
+  const int path = !near_rows(a, p.lda, M) || !near_rows(b, p.ldb, N) ? 2
+                   : aligned(a, p.lda, T) && aligned(b, p.ldb, T) &&
+                           M % epc == 0 && N % epc == 0 ? 0
+                   : 1;
   const int64_t k_tiles = T / E / (ty == GT_F32 ? 32 : 64);
-  const Plan plan = choose(ty, fast, k_tiles, [&](int64_t bm, int64_t bn) {
+  const Plan plan = choose(ty, path == 0, k_tiles, [&](int64_t bm, int64_t bn) {
     return E * ceil_div(M, bm) * ceil_div(N, bn);
   });
   const int tile = plan.tile;
   const hipStream_t s = stream_of(a);
   const Tensor part = begin(p, c, plan.splits);
-  if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, fast, s);
-  else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, fast, s);
-  else launch_grouped_f32(&p, tile, 0, 1, fast, s);
+  if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, path, s);
+  else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, path, s);
+  else launch_grouped_f32(&p, tile, 0, 1, path, s);
   finish(p, c, s);
   return c;
 }
@@ -319,14 +319,14 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   p.gsb = E > 1 ? N * K : 0;
   p.out = type_of(c.scalar_type());
   p.accum = accum;
-  p.near_a = near_rows(a, p.lda, K);
-  p.near_b = near_rows(bt, p.ldb, K);
-  const bool fast = p.near_a && p.near_b && aligned(a, p.lda, T) &&
-                    aligned(bt, p.ldb, N) && aligned(bt, p.gsb, E);
-  const Plan plan = choose_rows(GT_FP8, true, fast, T, E, K, N);
+  const int path = !near_rows(a, p.lda, K) || !near_rows(bt, p.ldb, K) ? 2
+                   : aligned(a, p.lda, T) && aligned(bt, p.ldb, N) &&
+                           aligned(bt, p.gsb, E) ? 0
+                   : 1;
+  const Plan plan = choose_rows(GT_FP8, true, path == 0, T, E, K, N);
   const hipStream_t s = stream_of(a);
   const Tensor part = begin(p, c, accum ? 1 : plan.splits);
-  launch_rows(p, GT_FP8, plan.tile, true, fast, s);
+  launch_rows(p, GT_FP8, plan.tile, true, path, s);
   finish(p, c, s);
   return c;
 }
@@ -347,8 +347,7 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x) {
               "matrix is too large");
   const int64_t ld = R > 1 ? x.stride(0) : 0;
   launch_fp8_quantize_row(x.data_ptr(), ty, ld, R, C, q.data_ptr(),
-                          s.data_ptr<float>(), aligned(x, ld, R),
-                          stream_of(x));
+                          s.data_ptr<float>(), stream_of(x));
   check_launch();
   return {q, s};
 }
@@ -383,7 +382,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
                            both ? qt.data_ptr() : nullptr,
                            s.data_ptr<float>(),
                            both ? st.data_ptr<float>() : nullptr,
-                           aligned(x, ld, R) && aligned(x, bld, E),
                            stream_of(x));
   check_launch();
   return {q, s, qt, st};

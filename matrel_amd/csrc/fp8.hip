@@ -20,25 +20,28 @@ template <int TY> __device__ __forceinline__ float load1(const void* x, long i) 
   return (float)((const _Float16*)x)[i];
 }
 
-// Eight neighbouring values, zeros from `have` on.
+// Eight neighbouring values from any address, zeros from `have` on.
 template <int TY>
 __device__ __forceinline__ void load8(const void* x, long i, int have,
-                                      bool vec, float* v) {
-  if (vec && have >= 8) {
+                                      float* v) {
+  if (have >= 8) {
     if constexpr (TY == GT_F32) {
-      const f32x4 lo = *(const f32x4*)((const float*)x + i);
-      const f32x4 hi = *(const f32x4*)((const float*)x + i + 4);
+      f32x4 lo, hi;
+      __builtin_memcpy(&lo, (const float*)x + i, 16);
+      __builtin_memcpy(&hi, (const float*)x + i + 4, 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[j] = lo[j];
         v[4 + j] = hi[j];
       }
     } else if constexpr (TY == GT_BF16) {
-      const bf16x8 q = *(const bf16x8*)((const __bf16*)x + i);
+      bf16x8 q;
+      __builtin_memcpy(&q, (const __bf16*)x + i, 16);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = (float)q[j];
     } else {
-      const f16x8 q = *(const f16x8*)((const _Float16*)x + i);
+      f16x8 q;
+      __builtin_memcpy(&q, (const _Float16*)x + i, 16);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = (float)q[j];
     }
@@ -57,10 +60,9 @@ __device__ __forceinline__ uint2 pack8(const float* v, float up) {
   return make_uint2((u32)lo, (u32)hi);
 }
 
-__device__ __forceinline__ void put8(unsigned char* o, uint2 q, int have,
-                                     bool vec) {
-  if (vec && have >= 8) {
-    *(uint2*)o = q;
+__device__ __forceinline__ void put8(unsigned char* o, uint2 q, int have) {
+  if (have >= 8) {
+    __builtin_memcpy(o, &q, 8);
     return;
   }
 #pragma unroll
@@ -75,15 +77,14 @@ __device__ __forceinline__ void put8(unsigned char* o, uint2 q, int have,
 template <int TY>
 __global__ void __launch_bounds__(256)
 quantize_row_k(const void* __restrict__ x, long ld, long rows, long cols,
-               unsigned char* __restrict__ q, float* __restrict__ scale,
-               int vec_in) {
+               unsigned char* __restrict__ q, float* __restrict__ scale) {
   const long ncb = (cols + 127) / 128, cb = blockIdx.x % ncb;
   const long row = blockIdx.x / ncb * 16 + (threadIdx.x >> 4);
   const long col = cb * 128 + (threadIdx.x & 15) * 8;
   const bool in = row < rows && col < cols;
   const int have = in ? (int)min(8L, cols - col) : 0;
   float v[8];
-  load8<TY>(x, in ? row * ld + col : 0, have, vec_in, v);
+  load8<TY>(x, in ? row * ld + col : 0, have, v);
   u32 top = TOP_MIN;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
@@ -91,7 +92,7 @@ quantize_row_k(const void* __restrict__ x, long ld, long rows, long cols,
   for (int d = 1; d < 16; d <<= 1) top = max(top, (u32)__shfl_xor((int)top, d));
   const float t = __uint_as_float(top);
   if (!in) return;
-  put8(q + row * cols + col, pack8(v, 448.0f / t), have, cols % 8 == 0);
+  put8(q + row * cols + col, pack8(v, 448.0f / t), have);
   if ((threadIdx.x & 15) == 0) scale[cb * rows + row] = t / 448.0f;
 }
 
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(256)
 quantize_tile_k(const void* __restrict__ x, long ld, long batch_ld, long rows,
                 long cols, unsigned char* __restrict__ q,
                 unsigned char* __restrict__ qt, float* __restrict__ scale,
-                float* __restrict__ scale_t, int vec_in) {
+                float* __restrict__ scale_t) {
   __shared__ u32 tops[4];
   __shared__ unsigned char turn[128][132];
   const long nrb = (rows + 127) / 128, ncb = (cols + 127) / 128;
@@ -117,7 +118,7 @@ quantize_tile_k(const void* __restrict__ x, long ld, long batch_ld, long rows,
     const long row = row0 + i * 16;
     const bool in = row < rows && col < cols;
     load8<TY>(base, in ? row * ld + col : 0, in ? (int)min(8L, cols - col) : 0,
-              vec_in, v[i]);
+              v[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
   }
@@ -136,8 +137,7 @@ quantize_tile_k(const void* __restrict__ x, long ld, long batch_ld, long rows,
     const long row = row0 + i * 16;
     const uint2 w = pack8(v[i], up);
     if (row < rows && col < cols)
-      put8(q + (e * rows + row) * cols + col, w, (int)min(8L, cols - col),
-           cols % 8 == 0);
+      put8(q + (e * rows + row) * cols + col, w, (int)min(8L, cols - col));
     if (qt) {
       u32* s = (u32*)&turn[(threadIdx.x >> 4) + i * 16][(threadIdx.x & 15) * 8];
       s[0] = w.x;
@@ -157,18 +157,17 @@ quantize_tile_k(const void* __restrict__ x, long ld, long batch_ld, long rows,
       w[j >> 2] |= (u32)turn[(threadIdx.x & 15) * 8 + j][c] << (8 * (j & 3));
     if (cb * 128 + c < cols && r8 < rows)
       put8(qt + (e * cols + cb * 128 + c) * rows + r8, make_uint2(w[0], w[1]),
-           (int)min(8L, rows - r8), rows % 8 == 0);
+           (int)min(8L, rows - r8));
   }
 }
 
 extern "C" void launch_fp8_quantize_row(const void* x, int ty, long ld,
                                         long rows, long cols, void* q,
-                                        float* scale, int vec,
-                                        hipStream_t s) {
+                                        float* scale, hipStream_t s) {
   const dim3 grid((unsigned)((cols + 127) / 128 * ((rows + 15) / 16)));
 #define GO(TY)                                                              \
   hipLaunchKernelGGL(quantize_row_k<TY>, grid, dim3(256), 0, s, x, ld, rows, \
-                     cols, (unsigned char*)q, scale, vec)
+                     cols, (unsigned char*)q, scale)
   if (ty == GT_F32) GO(GT_F32);
   else if (ty == GT_BF16) GO(GT_BF16);
   else GO(GT_F16);
@@ -178,14 +177,14 @@ extern "C" void launch_fp8_quantize_row(const void* x, int ty, long ld,
 extern "C" void launch_fp8_quantize_tile(const void* x, int ty, long ld,
                                          long batch_ld, long batch, long rows,
                                          long cols, void* q, void* qt,
-                                         float* scale, float* scale_t, int vec,
+                                         float* scale, float* scale_t,
                                          hipStream_t s) {
   const dim3 grid((unsigned)(((cols + 127) / 128) * ((rows + 127) / 128)),
                   (unsigned)batch);
 #define GO(TY)                                                               \
   hipLaunchKernelGGL(quantize_tile_k<TY>, grid, dim3(256), 0, s, x, ld,      \
                      batch_ld, rows, cols, (unsigned char*)q,                \
-                     (unsigned char*)qt, scale, scale_t, vec)
+                     (unsigned char*)qt, scale, scale_t)
   if (ty == GT_F32) GO(GT_F32);
   else if (ty == GT_BF16) GO(GT_BF16);
   else GO(GT_F16);

@@ -18,5 +18,4 @@ struct GroupedArgs {
   int splits;
   int out;            // GroupedType of c
   int accum;          // add to c (f32, one split)
-  int near_a, near_b;  // rows of 16 bytes or more, a tile within 31 bits
 };

@@ -3,8 +3,8 @@
 
 #define TY GT_BF16
 extern "C" void launch_grouped_bf16(const GroupedArgs* p, int tile, int bk,
-                                  int weights, int fast, hipStream_t s) {
-  if (weights) launch_weights_tile<TY>(*p, tile, fast, s);
-  else if (bk) launch_rows_tile<TY, true>(*p, tile, fast, s);
-  else launch_rows_tile<TY, false>(*p, tile, fast, s);
+                                  int weights, int path, hipStream_t s) {
+  if (weights) launch_weights_tile<TY>(*p, tile, path, s);
+  else if (bk) launch_rows_tile<TY, true>(*p, tile, path, s);
+  else launch_rows_tile<TY, false>(*p, tile, path, s);
 }

@@ -301,40 +301,36 @@ struct Side {
     }
   }
 
-  // Any tile, any alignment: through registers, zeros for k >= klim.
-  // Loads stay free of branches (one inside would wait for the one before):
-  // a chunk that ends early is read from further in front and shifted.
-  // near: a row has at least a chunk, and offsets fit 31 bits.
-  // PARTS: the last chunk of an R side's rows may be a part of one.
-  template <bool PARTS>
-  __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile, int klim,
-                                       bool near) const {
-    if (!near) {
-      load_slowly(w, tile, klim);
-      return;
-    }
+  // Any tile, any alignment: through registers. Nothing in load() depends on
+  // what it loads or branches, so that loads stay on their way: a chunk that
+  // ends early is read from further in front, and put() shifts it.
+  __device__ __forceinline__ void load(i32x4 (&w)[IT], int tile,
+                                       int klim) const {
     const int k1 = klim - k0 - tile * BKE;  // k of the tile that exist
     const char* s = base + (long)tile * (KROWS ? 128 : (long)BKE * ld * ES);
-    if (k1 >= BKE) {
 #pragma unroll
-      for (int i = 0; i < IT; ++i)  // global loads need no alignment
-        __builtin_memcpy(&w[i], s + at[i], 16);
-    } else {
-      int back[IT];
+    for (int i = 0; i < IT; ++i)  // global loads need no alignment
+      __builtin_memcpy(&w[i], s + ((long)at[i] - back(i, k1)), 16);
+  }
+
+  __device__ __forceinline__ int back(int i, int k1) const {
+    const int id = i * NT + (int)threadIdx.x;
+    if constexpr (KROWS)
+      return max(0, (((id & 7) ^ (id >> 4 & 7)) + 1) * EPC - k1) * ES;
+    else
+      return max(0, id / CPR + 1 - k1) * (int)ld * ES;
+  }
+
+  // Zeros for k >= klim. PARTS: the last chunk of an R side's rows may be a
+  // part of one.
+  template <bool PARTS>
+  __device__ __forceinline__ void put(char* lds, i32x4 (&w)[IT], int tile,
+                                      int klim) const {
+    const int k1 = klim - k0 - tile * BKE;
+    if (k1 < BKE) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const int id = i * NT + (int)threadIdx.x;
-        if constexpr (KROWS)
-          back[i] = max(0, (((id & 7) ^ (id >> 4 & 7)) + 1) * EPC - k1) * ES;
-        else
-          back[i] = max(0, id / CPR + 1 - k1) * (int)ld * ES;
-      }
-#pragma unroll
-      for (int i = 0; i < IT; ++i)
-        __builtin_memcpy(&w[i], s + ((long)at[i] - back[i]), 16);
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        if constexpr (KROWS) w[i] = shifted(w[i], back[i]);
+        if constexpr (KROWS) w[i] = shifted(w[i], back(i, k1));
         else if ((i * NT + (int)threadIdx.x) / CPR >= k1)
           w[i] = i32x4{0, 0, 0, 0};
       }
@@ -349,6 +345,9 @@ struct Side {
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      *(i32x4*)(lds + (i * NT + threadIdx.x) * 16) = w[i];
   }
 
   // The chunk without its first n bytes, zeros behind.
@@ -368,41 +367,28 @@ struct Side {
     return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
   }
 
-  __device__ __forceinline__ void load_slowly(i32x4 (&w)[IT], int tile,
-                                              int klim) const {
-    const E* s0 = (const E*)base;
-    for (int i = 0; i < IT; ++i) {
-      const int id = i * NT + (int)threadIdx.x;
+  // Rows shorter than a chunk or further apart than 31 bits: element by
+  // element, straight to LDS.
+  __device__ __forceinline__ void gather(char* lds, int tile, int klim) const {
+#pragma unroll 1
+    for (int id = threadIdx.x; id < IT * NT; id += NT) {
       int n;  // elements of the chunk that exist
       const E* s;
       if constexpr (KROWS) {
         const int row = id >> 3;
         const int k = tile * BKE + ((id & 7) ^ (row >> 1 & 7)) * EPC;
         n = row0 + row < rlim ? klim - k0 - k : 0;
-        s = s0 + (long)row * ld + k;
+        s = (const E*)base + (long)row * ld + k;
       } else {
         const int k = tile * BKE + id / CPR;
         const int row = swz(id % CPR, id / CPR) * EPC;
         n = k0 + k < klim ? rlim - row0 - row : 0;
-        s = s0 + (long)k * ld + row;
+        s = (const E*)base + (long)k * ld + row;
       }
-      w[i] = i32x4{0, 0, 0, 0};
-      for (int j = 0; j < EPC; ++j) {
-        if (j >= n) continue;
-        const int v = (int)((u32)s[j] << (j * ES % 4 * 8));
-        // selected, since a register cannot be indexed
-        if (j * ES / 4 == 0) w[i][0] |= v;
-        if (j * ES / 4 == 1) w[i][1] |= v;
-        if (j * ES / 4 == 2) w[i][2] |= v;
-        if (j * ES / 4 == 3) w[i][3] |= v;
-      }
+#pragma unroll 1
+      for (int j = 0; j < EPC; ++j)
+        ((E*)(lds + id * 16))[j] = j < n ? s[j] : (E)0;
     }
-  }
-
-  static __device__ __forceinline__ void put(char* lds, const i32x4 (&w)[IT]) {
-#pragma unroll
-    for (int i = 0; i < IT; ++i)
-      *(i32x4*)(lds + (i * NT + threadIdx.x) * 16) = w[i];
   }
 
   // The chunk of the fragment of rows [row, row + 16) (row: a multiple of 16)
@@ -537,16 +523,17 @@ template <bool WEIGHTS> struct Results {
 // ---- small and middle tiles ------------------------------------------------
 
 // BM x BN results a workgroup, its waves WM x WN. AK/BK: the operand has k
-// along its rows. WEIGHTS: the sum runs over a group's rows. FAST: rows (and
-// for an R side its length) are multiples of 16 bytes.
+// along its rows. WEIGHTS: the sum runs over a group's rows.
 //
 // D LDS stages: the copies of D - 1 K tiles are on their way at a time, since
 // a tile's products are shorter than the way to memory; one barrier a tile.
-// Operands that are not FAST, and a last tile that ends early, go through
-// registers instead: loaded before the products of the tile before, put into
-// LDS behind them.
+// ALIGNED: rows (and for an R side its length) are multiples of 16 bytes, and
+// whole tiles are copied to LDS; a last tile that ends early, and all tiles of
+// ANY rows, go through registers. SLOW: rows shorter than that.
+enum RowsPath { ALIGNED, ANY, SLOW };
+
 template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
-          bool WEIGHTS, bool FAST>
+          bool WEIGHTS, RowsPath PATH>
 __global__ void __launch_bounds__(64 * WM * WN, 2)  // waves a SIMD
 grouped_k(const GroupedArgs p) {
   constexpr int NT = 64 * WM * WN;
@@ -638,53 +625,85 @@ grouped_k(const GroupedArgs p) {
     sa.init(p.a, p.lda, w.m0, w.mend, w.kbeg);
     sb.init((const char*)p.b + (WEIGHTS ? 0 : (long)w.g * p.gsb * ES), p.ldb,
             w.n0, p.N, w.kbeg);
-    const int fast = FAST ? whole : 0;  // tiles that go straight to LDS
-    int next = 0, to = 0;               // the next copy and its stage
-    auto copy = [&]() {
-      const u32 lds = to * STAGE;
-      if constexpr (SCALES)
-        glds4(scale + (long)next * scale_step,
-              smem + lds + (BM + BN) * 128 + tid * 4);
-      sa.copy(smem, lds, next);
-      sb.copy(smem, lds + BM * 128, next);
-      ++next;
-      to = to == D - 1 ? 0 : to + 1;
+    struct Held {  // a tile on its way through registers
+      typename SA::Regs a;
+      typename SB::Regs b;
+      float scale;
     };
-    typename SA::Regs ra;
-    typename SB::Regs rb;
-    float rs = 0;
-    auto load = [&](int tile) {
-      if constexpr (SCALES) rs = scale[(long)tile * scale_step];
-      sa.template load<!FAST>(ra, tile, w.kend, p.near_a);
-      sb.template load<!FAST>(rb, tile, w.kend, p.near_b);
+    auto load = [&](Held& h, int tile) {
+      if constexpr (SCALES) h.scale = scale[(long)tile * scale_step];
+      sa.load(h.a, tile, w.kend);
+      sb.load(h.b, tile, w.kend);
     };
-    auto put = [&](int stage) {
+    auto put = [&](Held& h, int tile, int stage) {
       char* lds = smem + stage * STAGE;
-      SA::put(lds, ra);
-      SB::put(lds + BM * 128, rb);
-      if constexpr (SCALES) ((float*)(lds + (BM + BN) * 128))[tid] = rs;
+      sa.template put<PATH != ALIGNED>(lds, h.a, tile, w.kend);
+      sb.template put<PATH != ALIGNED>(lds + BM * 128, h.b, tile, w.kend);
+      if constexpr (SCALES) ((float*)(lds + (BM + BN) * 128))[tid] = h.scale;
     };
-    for (int i = 0; i < D - 1 && i < fast; ++i) copy();
-    if (fast == 0) {
-      load(0);
-      put(0);
-    }
-    int stage = 0;
-    for (int t = 0; t < tiles; ++t) {
-      // tile t is there when no more than the D - 2 behind it are missing
-      if (FAST && next < fast)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * OPS) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      if (next < fast) copy();
-      const int after = stage == D - 1 ? 0 : stage + 1;
-      const bool regs = t + 1 < tiles && t + 1 >= fast;
-      if (regs) load(t + 1);
-      products(smem + stage * STAGE);
-      if (regs) put(after);
-      stage = after;
+    if constexpr (PATH == ALIGNED) {
+      int next = 0, to = 0;  // the next copy and its stage
+      auto copy = [&]() {
+        const u32 lds = to * STAGE;
+        if constexpr (SCALES)
+          glds4(scale + (long)next * scale_step,
+                smem + lds + (BM + BN) * 128 + tid * 4);
+        sa.copy(smem, lds, next);
+        sb.copy(smem, lds + BM * 128, next);
+        ++next;
+        to = to == D - 1 ? 0 : to + 1;
+      };
+      for (int i = 0; i < D - 1 && i < whole; ++i) copy();
+      int stage = 0;
+      for (int t = 0; t < whole; ++t) {
+        // tile t is there when no more than the D - 2 behind it are missing
+        if (next < whole)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * OPS) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (next < whole) copy();
+        products(smem + stage * STAGE);
+        stage = stage == D - 1 ? 0 : stage + 1;
+      }
+      if (whole < tiles) {
+        Held h;
+        load(h, whole);
+        __syncthreads();
+        put(h, whole, 0);
+        __syncthreads();
+        products(smem);
+      }
+    } else if constexpr (PATH == ANY) {
+      // two stages in LDS and two tiles in registers: a load has the time of
+      // two tiles' products
+      Held h0, h1;
+      load(h0, 0);
+      if (tiles > 1) load(h1, 1);
+      put(h0, 0, 0);
+      auto step = [&](int t, int stage, Held& free, Held& next) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (t + 2 < tiles) load(free, t + 2);
+        products(smem + stage * STAGE);
+        if (t + 1 < tiles) put(next, t + 1, stage ^ 1);
+      };
+      for (int t = 0; t < tiles; t += 2) {
+        step(t, 0, h0, h1);
+        if (t + 1 < tiles) step(t + 1, 1, h1, h0);
+      }
+    } else {
+      for (int t = 0; t < tiles; ++t) {
+        sa.gather(smem, t, w.kend);
+        sb.gather(smem + BM * 128, t, w.kend);
+        if constexpr (SCALES)
+          ((float*)(smem + (BM + BN) * 128))[tid] =
+              scale[(long)t * scale_step];
+        __syncthreads();
+        products(smem);
+        __syncthreads();
+      }
     }
   }
 
@@ -895,16 +914,16 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
 #undef GB_WAIT
     if (whole * BKE < depth) {  // what is left of k
       __syncthreads();
-      typename SA::Regs r;
-      typename SB::Regs s;
-      a0.template load<false>(r, whole, w.kend, true);
-      SA::put(smem, r);
-      a1.template load<false>(r, whole, w.kend, true);
-      SA::put(smem + HALF, r);
-      b0.template load<false>(s, whole, w.kend, true);
-      SB::put(smem + 2 * HALF, s);
-      b1.template load<false>(s, whole, w.kend, true);
-      SB::put(smem + 3 * HALF, s);
+      typename SA::Regs r, r1;
+      typename SB::Regs s, s1;
+      a0.load(r, whole, w.kend);
+      a1.load(r1, whole, w.kend);
+      b0.load(s, whole, w.kend);
+      b1.load(s1, whole, w.kend);
+      a0.template put<false>(smem, r, whole, w.kend);
+      a1.template put<false>(smem + HALF, r1, whole, w.kend);
+      b0.template put<false>(smem + 2 * HALF, s, whole, w.kend);
+      b1.template put<false>(smem + 3 * HALF, s1, whole, w.kend);
       load_scales(whole);
       __syncthreads();
       take_scales();

@@ -2,7 +2,7 @@
 // row of a and each 128 x 128 tile of b.
 #include "grouped_launch.h"
 
-extern "C" void launch_grouped_fp8(const GroupedArgs* p, int tile, int fast,
+extern "C" void launch_grouped_fp8(const GroupedArgs* p, int tile, int path,
                                    hipStream_t s) {
-  launch_rows_tile<GT_FP8, true>(*p, tile, fast, s);
+  launch_rows_tile<GT_FP8, true>(*p, tile, path, s);
 }

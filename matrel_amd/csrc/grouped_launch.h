@@ -4,7 +4,7 @@
 #include "grouped_skinny.h"
 
 template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
-          bool WEIGHTS, bool FAST>
+          bool WEIGHTS, RowsPath PATH>
 static void grouped_go(const GroupedArgs& p, hipStream_t s) {
   const long ntn = (p.N + BN - 1) / BN;
   // every range of rows that is not empty can end inside one tile more
@@ -12,7 +12,7 @@ static void grouped_go(const GroupedArgs& p, hipStream_t s) {
                            : p.T / BM + p.E + 2;
   const size_t lds =
       D * ((BM + BN) * 128 + (TY == GT_FP8 ? WM * WN * 256 : 0));
-  auto k = grouped_k<TY, BM, BN, WM, WN, D, AK, BK, WEIGHTS, FAST>;
+  auto k = grouped_k<TY, BM, BN, WM, WN, D, AK, BK, WEIGHTS, PATH>;
   hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
                      dim3(64 * WM * WN), lds, s, p);
 }
@@ -32,38 +32,42 @@ static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
 //   0: 32 x 128   1: 64 x 64   2: 128 x 128   3: 256 x 256 (not f32)
 // Stages are as many as let two workgroups share the LDS of a CU.
 template <int TY, bool BK>
-static void launch_rows_tile(const GroupedArgs& p, int tile, bool fast,
+static void launch_rows_tile(const GroupedArgs& p, int tile, int path,
                              hipStream_t s) {
   if constexpr (BK) {
-    if (tile == -1) return grouped_skinny_go<TY, 1>(p, fast, s);
-    if (tile == -2) return grouped_skinny_go<TY, 2>(p, fast, s);
+    if (tile == -1) return grouped_skinny_go<TY, 1>(p, path == ALIGNED, s);
+    if (tile == -2) return grouped_skinny_go<TY, 2>(p, path == ALIGNED, s);
   }
-  if (!fast) {
+  if (path == SLOW)
+    return grouped_go<TY, 64, 64, 2, 2, 1, true, BK, false, SLOW>(p, s);
+  if (path == ANY) {
     if (tile == 2)
-      return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, false>(p, s);
-    return grouped_go<TY, 64, 64, 2, 2, 2, true, BK, false, false>(p, s);
+      return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, ANY>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 2, true, BK, false, ANY>(p, s);
   }
   if constexpr (TY != GT_F32)
     if (tile == 3) return grouped_big_go<TY, true, BK, false>(p, s);
   if (tile >= 2)
-    return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, true>(p, s);
+    return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, ALIGNED>(p, s);
   if (tile == 1)
-    return grouped_go<TY, 64, 64, 2, 2, 4, true, BK, false, true>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 4, true, BK, false, ALIGNED>(p, s);
   if constexpr (!BK)  // with k along b's rows, -1 and -2 take few rows
-    grouped_go<TY, 32, 128, 1, 4, 3, true, BK, false, true>(p, s);
+    grouped_go<TY, 32, 128, 1, 4, 3, true, BK, false, ALIGNED>(p, s);
 }
 
 template <int TY>
-static void launch_weights_tile(const GroupedArgs& p, int tile, bool fast,
+static void launch_weights_tile(const GroupedArgs& p, int tile, int path,
                                 hipStream_t s) {
-  if (!fast) {
+  if (path == SLOW)
+    return grouped_go<TY, 64, 64, 2, 2, 1, false, false, true, SLOW>(p, s);
+  if (path == ANY) {
     if (tile >= 2)
-      return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, false>(p, s);
-    return grouped_go<TY, 64, 64, 2, 2, 2, false, false, true, false>(p, s);
+      return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, ANY>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 2, false, false, true, ANY>(p, s);
   }
   if constexpr (TY != GT_F32)
     if (tile == 3) return grouped_big_go<TY, false, false, true>(p, s);
   if (tile >= 2)
-    return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, true>(p, s);
-  grouped_go<TY, 64, 64, 2, 2, 4, false, false, true, true>(p, s);
+    return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, ALIGNED>(p, s);
+  grouped_go<TY, 64, 64, 2, 2, 4, false, false, true, ALIGNED>(p, s);
 }
