@@ -2,6 +2,8 @@
 // Host-side only: what the kernels assume of shapes, strides and alignment is
 // checked or chosen here.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -65,6 +67,11 @@ bool aligned(const Tensor& t, int64_t ld, int64_t count) {
 bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
   return len * t.element_size() >= 16 &&
          ld * t.element_size() < (1 << 23);
+}
+
+// t, or a copy whose last dimension is contiguous.
+Tensor rows_contiguous(const Tensor& t) {
+  return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
 void set_offsets(GroupedArgs& p, c10::optional<Tensor>& offs,
@@ -159,7 +166,7 @@ void launch_rows(const GroupedArgs& p, int ty, int tile, bool bk, int path,
 }
 
 // c[t, :] = a[t, :] @ b[group of t], zeros for rows of no group.
-// a [T, K], last dimension contiguous; b [E, K, N], k or n contiguous.
+// a [T, K], b [E, K, N]; k or n of b contiguous, or it is copied.
 Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
                     at::ScalarType out) {
   TORCH_CHECK(a.is_cuda() && b.device() == a.device(),
@@ -179,10 +186,9 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   Tensor c = torch::empty({T, N}, a.options().dtype(out));
   if (c.numel() == 0) return c;
   if (E == 0 || K == 0) return c.zero_();
-  TORCH_CHECK(K == 1 || a.stride(1) == 1, "rows of a must be contiguous");
-  const bool bk = K == 1 || b.stride(1) == 1;
-  TORCH_CHECK(bk || N == 1 || b.stride(2) == 1,
-              "b must be contiguous along one of its matrix dimensions");
+  a = rows_contiguous(a);
+  bool bk = K == 1 || b.stride(1) == 1;
+  if (!bk && N > 1 && b.stride(2) != 1) b = b.contiguous();
   const int64_t epc = 16 / a.element_size();
   p.a = a.data_ptr();
   p.b = b.data_ptr();
@@ -205,7 +211,7 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
 }
 
 // c[g] = a_g^T @ b_g over the rows of each group, zeros for an empty one.
-// a [T, M], b [T, N], last dimensions contiguous.
+// a [T, M], b [T, N].
 Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
                        int64_t E, at::ScalarType out) {
   TORCH_CHECK(a.is_cuda() && b.device() == a.device(),
@@ -226,8 +232,8 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   Tensor c = torch::empty({E, M, N}, a.options().dtype(out));
   if (c.numel() == 0) return c;
   if (T == 0) return c.zero_();
-  TORCH_CHECK((M == 1 || a.stride(1) == 1) && (N == 1 || b.stride(1) == 1),
-              "rows must be contiguous");
+  a = rows_contiguous(a);
+  b = rows_contiguous(b);
   const int64_t epc = 16 / a.element_size();
   p.a = a.data_ptr();
   p.b = b.data_ptr();
@@ -336,7 +342,7 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2);
   const c10::hip::HIPGuard guard(x.device().index());
   const int64_t R = x.size(0), C = x.size(1);
-  TORCH_CHECK(C <= 1 || x.stride(1) == 1, "rows must be contiguous");
+  x = rows_contiguous(x);
   const int ty = type_of(x.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   Tensor q = torch::empty({R, C}, x.options().dtype(torch::kFloat8_e4m3fn));
@@ -359,7 +365,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
   TORCH_CHECK(x.is_cuda() && x.dim() == 3);
   const c10::hip::HIPGuard guard(x.device().index());
   const int64_t E = x.size(0), R = x.size(1), C = x.size(2);
-  TORCH_CHECK(C <= 1 || x.stride(2) == 1, "rows must be contiguous");
+  x = rows_contiguous(x);
   const int ty = type_of(x.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128;
@@ -387,6 +393,133 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
   return {q, s, qt, st};
 }
 
+// ---- autograd --------------------------------------------------------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that were computed outside of autograd: they say so when they are
+// differentiated once more.
+variable_list once(variable_list grads, bool create_graph) {
+  if (!create_graph) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_();
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "grouped and 8-bit products are differentiable once only",
+      (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+c10::optional<Tensor> given(const Tensor& offs) {
+  return offs.defined() ? c10::optional<Tensor>(offs) : c10::nullopt;
+}
+
+Tensor grad_a(const Tensor& grad, const Tensor& b,
+              const c10::optional<Tensor>& offs) {
+  return grouped_rows(grad, b.transpose(1, 2), offs, b.scalar_type());
+}
+
+// In the memory order of b, so that an optimizer walks both alike.
+Tensor grad_b(const Tensor& grad, const Tensor& a, const Tensor& b,
+              const c10::optional<Tensor>& offs) {
+  if (b.stride(1) == 1 && b.size(1) > 1)
+    return grouped_weights(grad, a, offs, b.size(0), b.scalar_type())
+        .transpose(1, 2);
+  return grouped_weights(a, grad, offs, b.size(0), b.scalar_type());
+}
+
+struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& a,
+                        const Tensor& b, const Tensor& offs, int64_t out) {
+    ctx->save_for_backward({a, b, offs});
+    return grouped_rows(a, b, offs, (at::ScalarType)out);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    const at::NoGradGuard guard;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &a = saved[0], &b = saved[1], &offs = saved[2];
+    // the products need one type: a float32 result of 16-bit operands rounds
+    // its gradient to theirs
+    const Tensor grad = rows_contiguous(grads[0].to(a.scalar_type()));
+    Tensor da, db;
+    if (ctx->needs_input_grad(0)) da = grad_a(grad, b, offs);
+    if (ctx->needs_input_grad(1)) db = grad_b(grad, a, b, offs);
+    auto r = once({da, db}, again);
+    return {r[0], r[1], Tensor(), Tensor()};
+  }
+};
+
+Tensor grouped_matmul(Tensor a, Tensor b, Tensor offs, at::ScalarType out) {
+  return GroupedMatmul::apply(a, b, offs, (int64_t)out);
+}
+
+// w [N, K] or [E, N, K], quantized here; or already quantized in q and s.
+struct Fp8Matmul : torch::autograd::Function<Fp8Matmul> {
+  typedef std::optional<Tensor> Maybe;
+  static Tensor forward(AutogradContext* ctx, const Tensor& a, const Maybe& w,
+                        const Maybe& q, const Maybe& s, const Maybe& offs,
+                        int64_t out) {
+    Tensor bt, bsc, turned, turned_sc;
+    ctx->saved_data["frozen"] = !w.has_value();
+    ctx->saved_data["a_type"] = (int64_t)a.scalar_type();
+    bool keep = false;
+    if (w.has_value()) {
+      std::tie(bt, bsc, turned, turned_sc) = fp8_quantize_tile(
+          w->dim() == 3 ? *w : w->unsqueeze(0), a.requires_grad());
+      ctx->saved_data["w_type"] = (int64_t)w->scalar_type();
+      ctx->saved_data["w_shape"] = w->sizes().vec();
+      keep = w->requires_grad();
+    } else {  // turned when the gradient is wanted
+      turned = bt = *q;
+      turned_sc = bsc = *s;
+    }
+    ctx->save_for_backward({keep ? a : Tensor(), turned, turned_sc,
+                            offs.has_value() ? *offs : Tensor()});
+    return grouped_rows_fp8(a, c10::nullopt, bt, bsc, offs,
+                            (at::ScalarType)out, c10::nullopt, false);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    const at::NoGradGuard guard;
+    const auto saved = ctx->get_saved_variables();
+    const auto a_type = (at::ScalarType)ctx->saved_data["a_type"].toInt();
+    const c10::optional<Tensor> offs = given(saved[3]);
+    const Tensor grad = rows_contiguous(grads[0]);
+    Tensor da, dw;
+    if (ctx->needs_input_grad(0)) {
+      Tensor bt = saved[1], bsc = saved[2];
+      if (ctx->saved_data["frozen"].toBool()) {
+        bt = bt.view(torch::kUInt8).transpose(-1, -2).contiguous().view(
+            torch::kFloat8_e4m3fn);
+        bsc = bsc.transpose(-1, -2).contiguous();
+      }
+      da = grouped_rows_fp8(grad, c10::nullopt, bt, bsc, offs, a_type,
+                            c10::nullopt, false);
+    }
+    if (!ctx->saved_data["frozen"].toBool() && ctx->needs_input_grad(1)) {
+      // in the operands' own type: the sum runs over rows, along which
+      // neither has its scales
+      const auto shape = ctx->saved_data["w_shape"].toIntVector();
+      dw = grouped_weights(rows_contiguous(grad.to(a_type)), saved[0], offs,
+                           shape.size() == 2 ? 1 : shape[0],
+                           (at::ScalarType)ctx->saved_data["w_type"].toInt())
+               .reshape(shape);
+    }
+    auto r = once({da, dw}, again);
+    return {r[0], r[1], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor fp8_matmul(Tensor a, c10::optional<Tensor> w, c10::optional<Tensor> q,
+                  c10::optional<Tensor> s, c10::optional<Tensor> offs,
+                  at::ScalarType out) {
+  TORCH_CHECK(w.has_value() || (q.has_value() && s.has_value()));
+  return Fp8Matmul::apply(a, w, q, s, offs, (int64_t)out);
+}
+
 // Whether an autograd graph that still lives accumulates into this leaf.
 bool has_grad_accumulator(const Tensor& t) {
   return t.requires_grad() && t.is_leaf() &&
@@ -406,5 +539,7 @@ void bind_grouped(pybind11::module& m) {
         "e4m3 with a scale for each 128 of a row");
   m.def("fp8_quantize_tile", &fp8_quantize_tile,
         "e4m3 with a scale for each 128 x 128 tile");
+  m.def("grouped_matmul", &grouped_matmul, "differentiable grouped_rows");
+  m.def("fp8_matmul", &fp8_matmul, "differentiable grouped_rows_fp8");
   m.def("has_grad_accumulator", &has_grad_accumulator);
 }

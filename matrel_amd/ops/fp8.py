@@ -22,7 +22,7 @@ import torch
 
 from .backend import require_ext, use_hip
 from .grouped import (check_capture, check_offsets, check_out_dtype,
-                      needs_grad, rows_contiguous, rows_product, weights_product)
+                      needs_grad, rows_product, weights_product)
 
 BLOCK = 128
 _MAX = 448.0
@@ -140,7 +140,6 @@ def quantize_fp8(x: torch.Tensor, kind: str = "row") -> Fp8Blocks:
     if not use_hip(x):
         return _cpu_quantize(x, kind)
     e = require_ext()
-    x = rows_contiguous(x)
     if kind == "tile":
         q, s, _, _ = e.fp8_quantize_tile(x if x.dim() == 3 else x[None],
                                          False)
@@ -166,55 +165,42 @@ def _product(a, bt: Fp8Blocks, offsets, out_dtype):
                             (w if w.dim() == 3 else w[None]).transpose(1, 2),
                             offsets, out_dtype)
     return require_ext().grouped_rows_fp8(
-        a.data if blocks else rows_contiguous(a),
+        a.data if blocks else a,
         a.scale if blocks else None, bt.data, bt.scale, offsets, out_dtype,
         None, False)
 
 
-def _quantize_both(w: torch.Tensor):
-    """(tiles of w, tiles of w^T) in one pass; w [groups, n, k]."""
-    if not use_hip(w):
-        q = _cpu_quantize(w, "tile")
-        return q, q.transpose()
-    q, s, qt, st = require_ext().fp8_quantize_tile(rows_contiguous(w), True)
-    return Fp8Blocks._made(q, s, "tile"), Fp8Blocks._made(qt, st, "tile")
+class _CpuFp8Matmul(torch.autograd.Function):
+    """Fp8Matmul of csrc/ext_grouped.cpp for CPU tensors."""
 
-
-class _Fp8Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, w, frozen, offsets, out_dtype):
-        w3 = None if w is None else (w if w.dim() == 3 else w[None])
-        turned = None
-        if w is None:
-            q = frozen
-        elif ctx.needs_input_grad[0]:
-            q, turned = _quantize_both(w3)
-        else:
-            q = quantize_fp8(w3, "tile")
-        ctx.turned, ctx.frozen = turned, None if w is not None else q
-        ctx.w = None if w is None else (w.shape, w.dtype)
-        ctx.a_dtype = a.dtype
-        ctx.save_for_backward(
-            a if ctx.needs_input_grad[1] else None, offsets)
+        q = _cpu_quantize(w, "tile") if frozen is None else frozen
+        ctx.q, ctx.frozen = q, frozen is not None
+        ctx.save_for_backward(a, w, offsets)
         return _product(a, q, offsets, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        a, offsets = ctx.saved_tensors
+        a, w, offsets = ctx.saved_tensors
         da = dw = None
         if ctx.needs_input_grad[0]:
-            turned = ctx.turned if ctx.turned is not None \
-                else ctx.frozen.transpose()
-            da = _product(grad, turned, offsets, ctx.a_dtype)
-        if ctx.needs_input_grad[1]:
+            da = _product(grad, ctx.q.transpose(), offsets, a.dtype)
+        if not ctx.frozen and ctx.needs_input_grad[1]:
             # in the operands' own type: the sum runs over rows, along which
             # neither has its scales
-            shape, dtype = ctx.w
-            groups = 1 if len(shape) == 2 else shape[0]
-            dw = weights_product(grad.to(a.dtype), a, offsets, groups, dtype)
-            dw = dw.reshape(shape)
+            groups = 1 if w.dim() == 2 else w.shape[0]
+            dw = weights_product(grad.to(a.dtype), a, offsets, groups,
+                                 w.dtype).reshape(w.shape)
         return da, dw, None, None, None
+
+
+def _differentiable(a, w, frozen, offsets, out_dtype):
+    if not use_hip(a):
+        return _CpuFp8Matmul.apply(a, w, frozen, offsets, out_dtype)
+    q, s = (None, None) if frozen is None else (frozen.data, frozen.scale)
+    return require_ext().fp8_matmul(a, w, q, s, offsets, out_dtype)
 
 
 def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
@@ -266,9 +252,9 @@ def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
             raise TypeError(f"a is {a.dtype}, bt {bt.dtype}")
         if needs_grad(a, bt):
             check_capture(a, bt)
-            return _Fp8Matmul.apply(a, bt, None, offsets, out_dtype)
+            return _differentiable(a, bt, None, offsets, out_dtype)
         bt = quantize_fp8(bt, "tile")
     elif needs_grad(a):
         check_capture(a)
-        return _Fp8Matmul.apply(a, None, bt, offsets, out_dtype)
+        return _differentiable(a, None, bt, offsets, out_dtype)
     return _product(a, bt, offsets, out_dtype)

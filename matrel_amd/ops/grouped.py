@@ -73,17 +73,6 @@ def check_capture(*leaves) -> None:
                 "capturing, or capture grouped_matmul_grads instead")
 
 
-def rows_contiguous(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy whose last dimension is contiguous."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def _matrix_contiguous(b: torch.Tensor) -> torch.Tensor:
-    if 1 in (b.stride(1), b.stride(2)) or 1 in b.shape[1:]:
-        return b
-    return b.contiguous()
-
-
 def _cpu_rows(a, b, offsets, out_dtype):
     out = torch.zeros(a.shape[0], b.shape[2])
     v = [0, a.shape[0]] if offsets is None else offsets.tolist()
@@ -104,16 +93,14 @@ def rows_product(a, b, offsets, out_dtype):
     """c[t] = a[t] @ b[group of t]; offsets None: one group of all rows."""
     if not use_hip(a):
         return _cpu_rows(a, b, offsets, out_dtype)
-    return require_ext().grouped_rows(
-        rows_contiguous(a), _matrix_contiguous(b), offsets, out_dtype)
+    return require_ext().grouped_rows(a, b, offsets, out_dtype)
 
 
 def weights_product(a, b, offsets, groups, out_dtype):
     """c[g] = a_g^T @ b_g over the rows of each group."""
     if not use_hip(a):
         return _cpu_weights(a, b, offsets, groups, out_dtype)
-    return require_ext().grouped_weights(
-        rows_contiguous(a), rows_contiguous(b), offsets, groups, out_dtype)
+    return require_ext().grouped_weights(a, b, offsets, groups, out_dtype)
 
 
 def _check(a, b, offsets):
@@ -163,7 +150,9 @@ def _grad_b(grad, a, b, offsets):
     return weights_product(a, grad, offsets, b.shape[0], b.dtype)
 
 
-class _GroupedMatmul(torch.autograd.Function):
+class _CpuGroupedMatmul(torch.autograd.Function):
+    """GroupedMatmul of csrc/ext_grouped.cpp for CPU tensors."""
+
     @staticmethod
     def forward(ctx, a, b, offsets, out_dtype):
         ctx.save_for_backward(a, b, offsets)
@@ -196,5 +185,7 @@ def grouped_matmul(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     out_dtype = check_out_dtype(out_dtype, a.dtype)
     if not needs_grad(a, b):
         return rows_product(a, b, offsets, out_dtype)
+    if not use_hip(a):
+        return _CpuGroupedMatmul.apply(a, b, offsets, out_dtype)
     check_capture(a, b)
-    return _GroupedMatmul.apply(a, b, offsets, out_dtype)
+    return require_ext().grouped_matmul(a, b, offsets, out_dtype)
