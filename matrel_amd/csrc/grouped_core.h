@@ -653,6 +653,7 @@ grouped_k(const GroupedArgs p) {
         ++next;
         to = to == D - 1 ? 0 : to + 1;
       };
+      Held h;
       for (int i = 0; i < D - 1 && i < whole; ++i) copy();
       int stage = 0;
       for (int t = 0; t < whole; ++t) {
@@ -664,16 +665,15 @@ grouped_k(const GroupedArgs p) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         if (next < whole) copy();
+        if (t + 1 == whole && whole < tiles) load(h, whole);
         products(smem + stage * STAGE);
         stage = stage == D - 1 ? 0 : stage + 1;
       }
-      if (whole < tiles) {
-        Held h;
-        load(h, whole);
+      if (whole < tiles) {  // behind D - 1 others, its stage is free
+        if (whole == 0) load(h, 0);
+        put(h, whole, stage);
         __syncthreads();
-        put(h, whole, 0);
-        __syncthreads();
-        products(smem);
+        products(smem + stage * STAGE);
       }
     } else if constexpr (PATH == ANY) {
       // two stages in LDS and two tiles in registers: a load has the time of
@@ -726,6 +726,8 @@ grouped_k(const GroupedArgs p) {
 // younger copies in flight. The copies are never waited for to the last one
 // inside the loop. The second four waves have the higher priority: two waves
 // of a SIMD then take turns at the matrix unit instead of reading LDS at once.
+// A tile whose group ends within its first 128 rows does the first two phases
+// only.
 template <int TY, bool AK, bool BK, bool WEIGHTS>
 __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
   constexpr int ES = Elt<TY>::ES, BKE = 128 / ES;
@@ -861,8 +863,11 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     //   end of phase 1: B1 A1 S' A0'        B1 has to be there
     //   end of phase 2: A1 S' A0' B0'       A1 has to be there
     //   end of phase 4: S' A0' B0' B1' A1'  A0' and B0' have to be there
-#define GB_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
-    auto step = [&](auto more, int t) {
+#define GB_WAIT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+    // with the first rows alone:
+    //   end of phase 1: B1 S' A0'           B1 has to be there
+    //   end of phase 2: S' A0' B0' B1'      A0' and B0' have to be there
+    auto step = [&](auto more, auto both, int t) {
       const char* cur = smem + (t & 1) * BUF;
       const u32 nxt = (~t & 1) * BUF;
       take_scales();
@@ -873,25 +878,26 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
         a0.copy(smem, nxt, at(t + 1));
       }
       quarter(0, 0);
-      if constexpr (!more) GB_WAIT(2);
-      else if constexpr (TY == GT_FP8) GB_WAIT(8);
-      else GB_WAIT(4);
+      if constexpr (!more) GB_WAIT(both ? 2 : 0);
+      else GB_WAIT((both ? 4 : 2) + (TY == GT_FP8 ? 4 : 0));
       __builtin_amdgcn_s_barrier();
       read_b(cur, 1);
       if constexpr (more) b0.copy(smem, nxt + 2 * HALF, at(t + 1));
+      if constexpr (more && !both) b1.copy(smem, nxt + 3 * HALF, at(t + 1));
       quarter(0, 1);
-      if constexpr (!more) GB_WAIT(0);
-      else if constexpr (TY == GT_FP8) GB_WAIT(8);
-      else GB_WAIT(4);
-      __builtin_amdgcn_s_barrier();
-      read_a(cur, 1);
-      if constexpr (more) b1.copy(smem, nxt + 3 * HALF, at(t + 1));
-      quarter(1, 1);
-      read_b(cur, 0);
-      if constexpr (more) a1.copy(smem, nxt + HALF, at(t + 1));
-      quarter(1, 0);
+      if constexpr (both) {
+        if constexpr (!more) GB_WAIT(0);
+        else GB_WAIT(4 + (TY == GT_FP8 ? 4 : 0));
+        __builtin_amdgcn_s_barrier();
+        read_a(cur, 1);
+        if constexpr (more) b1.copy(smem, nxt + 3 * HALF, at(t + 1));
+        quarter(1, 1);
+        read_b(cur, 0);
+        if constexpr (more) a1.copy(smem, nxt + HALF, at(t + 1));
+        quarter(1, 0);
+      }
       // every read of this buffer is back too, before it is copied into
-      if constexpr (more) GB_WAIT(4);
+      if constexpr (more) GB_WAIT(both ? 4 : 2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
     };
@@ -900,16 +906,21 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
 
     if (__builtin_amdgcn_readfirstlane(threadIdx.x) >= 256)
       __builtin_amdgcn_s_setprio(1);
-    if (whole > 0) {
+    const bool lower = w.m0 + 128 < w.mend;
+    auto all = [&](auto both) {
       load_scales(at(0));
       a0.copy(smem, 0, at(0));
       b0.copy(smem, 2 * HALF, at(0));
       b1.copy(smem, 3 * HALF, at(0));
-      a1.copy(smem, HALF, at(0));
-      GB_WAIT(4);
+      if constexpr (both) a1.copy(smem, HALF, at(0));
+      GB_WAIT(both ? 4 : 2);
       __builtin_amdgcn_s_barrier();
-      for (int t = 0; t + 1 < whole; ++t) step(Yes{}, t);
-      step(No{}, whole - 1);
+      for (int t = 0; t + 1 < whole; ++t) step(Yes{}, both, t);
+      step(No{}, both, whole - 1);
+    };
+    if (whole > 0) {
+      if (lower) all(Yes{});
+      else all(No{});
     }
 #undef GB_WAIT
     if (whole * BKE < depth) {  // what is left of k
