@@ -30,7 +30,10 @@ static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
 // Tile codes, as choose_tile (ext_grouped.cpp) picks them.
 //   -1, -2: 16, 32 rows, columns by 16 (b with k along its rows)
 //   0: 32 x 128   1: 64 x 64   2: 128 x 128   3: 256 x 256 (not f32)
-// Stages are as many as let two workgroups share the LDS of a CU.
+// Stages: as many as let two workgroups (64 x 64: three) share a CU's LDS.
+// More stages for fewer workgroups lost: bf16 8192 rows, 8 groups, 4096 x 2048,
+// 128 x 128 with 2 / 4 stages: 169 / 229 us; f32 4096 rows, 12 groups, 1024 x
+// 1000, 64 x 64 with 3 / 4: 93 / 98 us.
 template <int TY, bool BK>
 static void launch_rows_tile(const GroupedArgs& p, int tile, int path,
                              hipStream_t s) {
@@ -50,7 +53,7 @@ static void launch_rows_tile(const GroupedArgs& p, int tile, int path,
   if (tile >= 2)
     return grouped_go<TY, 128, 128, 2, 2, 2, true, BK, false, ALIGNED>(p, s);
   if (tile == 1)
-    return grouped_go<TY, 64, 64, 2, 2, 4, true, BK, false, ALIGNED>(p, s);
+    return grouped_go<TY, 64, 64, 2, 2, 3, true, BK, false, ALIGNED>(p, s);
   if constexpr (!BK)  // with k along b's rows, -1 and -2 take few rows
     grouped_go<TY, 32, 128, 1, 4, 3, true, BK, false, ALIGNED>(p, s);
 }
@@ -69,5 +72,5 @@ static void launch_weights_tile(const GroupedArgs& p, int tile, int path,
     if (tile == 3) return grouped_big_go<TY, false, false, true>(p, s);
   if (tile >= 2)
     return grouped_go<TY, 128, 128, 2, 2, 2, false, false, true, ALIGNED>(p, s);
-  grouped_go<TY, 64, 64, 2, 2, 4, false, false, true, ALIGNED>(p, s);
+  grouped_go<TY, 64, 64, 2, 2, 3, false, false, true, ALIGNED>(p, s);
 }
