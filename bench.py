@@ -39,7 +39,7 @@ def main():
                     help="override matrix side N")
     ap.add_argument("--block-size", type=int, default=0,
                     help="0 = auto (single block at 1 GPU, 16384 for SUMMA)")
-    ap.add_argument("--precision", choices=["bf16", "mx8", "mx6", "mx4"],
+    ap.add_argument("--precision", choices=["bf16", "mx8", "mx6", "mx4", "fp8"],
                     default="bf16",
                     help="GEMM compute precision (mx8 = MX-scaled fp8; "
                          "NOT the headline config - BASELINE is bf16)")

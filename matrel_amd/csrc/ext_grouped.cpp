@@ -520,10 +520,15 @@ Tensor fp8_matmul(Tensor a, c10::optional<Tensor> w, c10::optional<Tensor> q,
   return Fp8Matmul::apply(a, w, q, s, offs, (int64_t)out);
 }
 
-// Whether an autograd graph that still lives accumulates into this leaf.
-bool has_grad_accumulator(const Tensor& t) {
-  return t.requires_grad() && t.is_leaf() &&
-         torch::autograd::impl::try_get_grad_accumulator(t) != nullptr;
+// Whether an autograd graph that met this leaf on another stream than the
+// current one still lives.
+bool held_by_other_stream(const Tensor& t) {
+  if (!t.requires_grad() || !t.is_leaf()) return false;
+  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!held || held->num_inputs() == 0) return false;
+  // by id: the one is of device type "cuda", the other "hip"
+  return held->input_metadata(0).stream().id() !=
+         c10::hip::getCurrentHIPStream(t.device().index()).id();
 }
 
 }  // namespace
@@ -541,5 +546,5 @@ void bind_grouped(pybind11::module& m) {
         "e4m3 with a scale for each 128 x 128 tile");
   m.def("grouped_matmul", &grouped_matmul, "differentiable grouped_rows");
   m.def("fp8_matmul", &fp8_matmul, "differentiable grouped_rows_fp8");
-  m.def("has_grad_accumulator", &has_grad_accumulator);
+  m.def("held_by_other_stream", &held_by_other_stream);
 }

@@ -79,10 +79,14 @@ def _bt_cached(b: BlockMatrix, k: int, bj: int,
     return bt
 
 
-_MXQ_PRECS = ("mx8", "mx6", "mx4")
+_MXQ_PRECS = ("mx8", "mx6", "mx4", "fp8")
 
 
-def _mxq_convert(prec: str, t: torch.Tensor):
+def _mxq_convert(prec: str, t: torch.Tensor, side: str):
+    """Payload and scales of an operand; side "a" or "b" (transposed): fp8
+    scales the one by rows, the other by tiles."""
+    if prec == "fp8":
+        return blockops.to_fp8(t, "row" if side == "a" else "tile")
     if prec == "mx4":
         return blockops.to_mx4(t)
     if prec == "mx6":
@@ -91,7 +95,9 @@ def _mxq_convert(prec: str, t: torch.Tensor):
 
 
 def _mxq_gemm(prec: str, c, a_p, a_sc, bt_p, bt_sc, beta0: bool) -> None:
-    if prec == "mx4":
+    if prec == "fp8":
+        blockops.gemm_bt_fp8_acc(c, a_p, a_sc, bt_p, bt_sc, beta0=beta0)
+    elif prec == "mx4":
         blockops.gemm_bt_mx4_acc(c, a_p, a_sc, bt_p, bt_sc, beta0=beta0)
     elif prec == "mx6":
         blockops.gemm_bt_mx6_acc(c, a_p, a_sc, bt_p, bt_sc, beta0=beta0)
@@ -108,8 +114,18 @@ def _mxq_pbytes(prec, bs: int) -> int:
     return bs
 
 
+def _mxq_panel_scales(prec, n: int, bs: int, side: str,
+                      device: torch.device) -> torch.Tensor:
+    """Room for the scales of n bs x bs panels: packed e8m0 words for the MX
+    tiers, float32 for fp8 (as _mxq_convert lays them out)."""
+    if prec == "fp8":
+        return torch.empty(n, bs // 128, bs if side == "a" else bs // 128,
+                           dtype=torch.float32, device=device)
+    return torch.empty(n, bs // 128, bs, dtype=torch.int32, device=device)
+
+
 def _mx8_cached(m: BlockMatrix, key, tensor_bf16: torch.Tensor,
-                prec: str = "mx8"):
+                prec: str = "mx8", side: str = "a"):
     """Per-matrix cache of MX-fp8/fp4 conversions (payloads are 1/2 or
     1/4 the bf16 bytes; reused across every multiply touching the
     block)."""
@@ -119,7 +135,7 @@ def _mx8_cached(m: BlockMatrix, key, tensor_bf16: torch.Tensor,
     key = (prec,) + (key if isinstance(key, tuple) else (key,))
     ent = cache.get(key)
     if ent is None:
-        ent = _mxq_convert(prec, tensor_bf16)
+        ent = _mxq_convert(prec, tensor_bf16, side)
         if _cache_has_headroom(sum(t.numel() * t.element_size()
                                    for t in ent)):
             cache[key] = ent
@@ -131,6 +147,9 @@ def _mx8_usable(t: torch.Tensor, prec: str = "mx8") -> bool:
     # the packed-scale mx6/mx4 converters and their k128 kernels need
     # cols % 128 (a ragged edge of width 64 mod 128 passes the mx8 rule
     # but raises in mx6_convert - caught by the refinement example).
+    # fp8 takes any shape.
+    if prec == "fp8":
+        return t.is_cuda and t.dtype == torch.bfloat16
     kmod = 32 if prec == "mx8" else 128
     return (t.is_cuda and t.dtype == torch.bfloat16
             and t.shape[0] % 256 == 0 and t.shape[1] % kmod == 0)
@@ -204,7 +223,7 @@ def _pad_t(t: torch.Tensor, bs: int) -> torch.Tensor:
 
 
 def _mx8_padded(m: BlockMatrix, key, t: torch.Tensor, bs: int,
-                prec: str = "mx8"):
+                prec: str = "mx8", side: str = "a"):
     """Cached MX-fp8/fp4 conversion of a (zero-padded) block."""
     cache = getattr(m, "_mx8_cache", None)
     if cache is None:
@@ -212,7 +231,7 @@ def _mx8_padded(m: BlockMatrix, key, t: torch.Tensor, bs: int,
     key = (prec,) + (key if isinstance(key, tuple) else (key,))
     ent = cache.get(key)
     if ent is None:
-        ent = _mxq_convert(prec, _pad_t(blockops.densify(t), bs))
+        ent = _mxq_convert(prec, _pad_t(blockops.densify(t), bs), side)
         if _cache_has_headroom(sum(x.numel() * x.element_size()
                                    for x in ent)):
             cache[key] = ent
@@ -402,10 +421,9 @@ def local_matmul(a: BlockMatrix, b: BlockMatrix, out: BlockMatrix) -> None:
                 continue
             bbd = blockops.densify(bb)
             bt = _bt_cached(b, k, bj, bbd)
-            if mx8 and _mx8_usable(ab, mxq) and _mx8_usable(bt, mxq) \
-                    and ab.shape[0] % 256 == 0 and bt.shape[0] % 256 == 0:
+            if mx8 and _mx8_usable(ab, mxq) and _mx8_usable(bt, mxq):
                 a8, asc = _mx8_cached(a, (bi, k), ab, mxq)
-                bt8, btsc = _mx8_cached(b, ("t", k, bj), bt, mxq)
+                bt8, btsc = _mx8_cached(b, ("t", k, bj), bt, mxq, "b")
                 _mxq_gemm(mxq, c, a8, asc, bt8, btsc, beta0=first)
                 continue
             if use_fused and last:
@@ -526,8 +544,8 @@ def summa_matmul(a: BlockMatrix, b: BlockMatrix, out: BlockMatrix) -> None:
                 a_stack = torch.empty(len(a_rows), bs, pbytes,
                                       dtype=torch.uint8, device=a.device)
                 # packed-dword scales [bs/128][bs] int32 (mxconvert r2)
-                a_sc = torch.empty(len(a_rows), bs // 128, bs,
-                                   dtype=torch.int32, device=a.device)
+                a_sc = _mxq_panel_scales(mxq, len(a_rows), bs, "a",
+                                         a.device)
                 _prep_reg(a_stack, a_sc)
                 if rt.rank == a_src:
                     with _prep_ctx():
@@ -647,8 +665,8 @@ def summa_matmul(a: BlockMatrix, b: BlockMatrix, out: BlockMatrix) -> None:
             if mx8:
                 b_stack = torch.empty(len(b_cols), bs, pbytes,
                                       dtype=torch.uint8, device=b.device)
-                b_sc = torch.empty(len(b_cols), bs // 128, bs,
-                                   dtype=torch.int32, device=b.device)
+                b_sc = _mxq_panel_scales(mxq, len(b_cols), bs, "b",
+                                         b.device)
                 _prep_reg(b_stack, b_sc)
                 if rt.rank == b_src:
                     with _prep_ctx():
@@ -657,7 +675,7 @@ def summa_matmul(a: BlockMatrix, b: BlockMatrix, out: BlockMatrix) -> None:
                                 b.get_block_dense(k, j)), bs)
                             p8, sc = _mx8_padded(b, ("st", k, j),
                                                  blockops.transpose(t),
-                                                 bs, mxq)
+                                                 bs, mxq, "b")
                             b_stack[n] = p8
                             b_sc[n] = sc
                     _prep_done()

@@ -372,3 +372,20 @@ def gemm_bt_mx8_acc(acc: torch.Tensor, a8, asc, bt8, btsc,
     scaled MFMA (~2x the bf16 rate). Shapes must satisfy M,N % 256 == 0,
     K % 64 == 0 (callers guard and fall back to bf16)."""
     require_ext().gemm_bt_mx8_acc(acc, a8, asc, bt8, btsc, beta0)
+
+
+def to_fp8(t: torch.Tensor, kind: str):
+    """(e4m3 bytes, float32 scales for each 128 of a row or 128 x 128 tile) of
+    a block; any shape (see ops/fp8.py)."""
+    from .fp8 import quantize_fp8
+    q = quantize_fp8(t, kind)
+    return q.data.view(torch.uint8), q.scale
+
+
+def gemm_bt_fp8_acc(acc: torch.Tensor, a8, asc, bt8, btsc,
+                    beta0: bool = False) -> None:
+    """acc(fp32) += dequant(a8,asc) @ dequant(bt8,btsc)^T via the 8-bit MFMA
+    with float32 block scales: a by rows, bt by tiles (to_fp8)."""
+    f8 = torch.float8_e4m3fn
+    require_ext().grouped_rows_fp8(a8.view(f8), asc, bt8.view(f8), btsc, None,
+                                   torch.float32, acc, not beta0)

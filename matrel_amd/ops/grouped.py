@@ -66,7 +66,7 @@ def check_capture(*leaves) -> None:
             or not torch.cuda.is_current_stream_capturing():
         return
     for t in leaves:
-        if require_ext().has_grad_accumulator(t):
+        if require_ext().held_by_other_stream(t):
             raise RuntimeError(
                 "an autograd graph built outside of this capture still "
                 "holds an operand: free it (its loss and outputs) before "
