@@ -571,7 +571,8 @@ grouped_k(const GroupedArgs p) {
     const bool rows = tid < BM;
     scale = rows ? p.asc + kb * p.T + min(w.m0 + tid, p.T - 1)
                  : p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
-                            kb) * nb + w.n0 / 128;
+                            kb) * nb +
+                       min(w.n0 / 128 + (tid & (BN / 128 - 1)), nb - 1);
     scale_step = rows ? p.T : nb;
   }
 
@@ -586,7 +587,7 @@ grouped_k(const GroupedArgs p) {
       i32x8 y[FM];
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        s[i] = sc[wm + i * 16 + (lane & 15)] * sc[BM];
+        s[i] = sc[wm + i * 16 + (lane & 15)] * sc[BM + wn / 128];
         y[i] = join8(SA::frag(la, wm + i * 16, 0),
                      SA::frag(la, wm + i * 16, 1));
       }
@@ -749,36 +750,26 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
   const int depth = w.kend - w.kbeg;
   const int whole = depth / BKE;
 
-  // fp8: scales of the wave's rows in both halves; of its columns uniform
-  u32 arow[2][2];
-  const float* asc = nullptr;
-  const float* bsc[2] = {nullptr, nullptr};
-  float ra[2][2], rb[2];
-  int nb = 0;
+  // fp8: the scales of a K tile go through LDS as well, a word a lane: of 256
+  // rows by the first four waves, of the two column blocks by the others.
+  // (Loaded into registers, they would be waited for together with all copies
+  // behind them.)
+  constexpr int SCALES = TY == GT_FP8 ? 2048 : 0;
+  const float* scale = nullptr;
+  int scale_step = 0;
   if constexpr (TY == GT_FP8) {
-    nb = (p.N + 127) / 128;
+    const int nb = (p.N + 127) / 128, tid = threadIdx.x;
     const long kb = w.kbeg / 128;
-    asc = p.asc + kb * p.T;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        arow[h][i] =
-            min(w.m0 + h * 128 + qr + i * 16 + (lane & 15), p.T - 1);
-      bsc[h] = p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
-                        kb) * nb + min(w.n0 / 128 + h, nb - 1);
-    }
+    scale = tid < 256
+                ? p.asc + kb * p.T + min(w.m0 + tid, p.T - 1)
+                : p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
+                           kb) * nb + min(w.n0 / 128 + (tid & 1), nb - 1);
+    scale_step = tid < 256 ? p.T : nb;
   }
-  auto load_scales = [&](int tile) {
-    if constexpr (TY == GT_FP8) {
-      const float* s = asc + (long)tile * p.T;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ra[h][i] = s[arow[h][i]];
-        rb[h] = bsc[h][(long)tile * nb];
-      }
-    }
+  auto copy_scales = [&](int stage, int tile) {
+    if constexpr (SCALES)
+      glds4(scale + (long)tile * scale_step,
+            smem + 2 * BUF + stage * SCALES + threadIdx.x * 4);
   };
 
   i32x4 y[2][2], x[2][4];  // [half of k][fragments]
@@ -796,12 +787,12 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       for (int j = 0; j < 4; ++j)
         x[kk][j] = SB::frag(buf + (2 + h) * HALF, qc + j * 16, kk);
   };
-  float sa_[2][2], sb_[2];  // the scales of the tile that is multiplied
+  float sa[2][2], sb[2];  // the scales of the tile that is multiplied
   auto quarter = [&](int hm, int hn) {
     if constexpr (TY == GT_FP8) {
       float sc[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc[i] = sa_[hm][i] * sb_[hn];
+      for (int i = 0; i < 2; ++i) sc[i] = sa[hm][i] * sb[hn];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -825,13 +816,15 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
                 mma<TY>(x[kk][j], y[kk][i], acc[hm][hn][j][i]);
     }
   };
-  auto take_scales = [&]() {
-    if constexpr (TY == GT_FP8) {
+  auto read_scales = [&](int stage) {
+    if constexpr (SCALES) {
+      const float* v = (const float*)(smem + 2 * BUF + stage * SCALES);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        sa_[h][0] = ra[h][0];
-        sa_[h][1] = ra[h][1];
-        sb_[h] = rb[h];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          sa[h][i] = v[h * 128 + qr + i * 16 + (lane & 15)];
+        sb[h] = v[256 + h];
       }
     }
   };
@@ -859,7 +852,7 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     };
 
     // vector memory operations of a lane in flight at each wait, oldest
-    // first (2 a half; S: the scales of fp8, 4 or more; ' = next tile):
+    // first (2 a half; S: the scales of fp8, 1; ' = next tile):
     //   end of phase 1: B1 A1 S' A0'        B1 has to be there
     //   end of phase 2: A1 S' A0' B0'       A1 has to be there
     //   end of phase 4: S' A0' B0' B1' A1'  A0' and B0' have to be there
@@ -870,16 +863,16 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     auto step = [&](auto more, auto both, int t) {
       const char* cur = smem + (t & 1) * BUF;
       const u32 nxt = (~t & 1) * BUF;
-      take_scales();
+      read_scales(t & 1);
       read_a(cur, 0);
       read_b(cur, 0);
       if constexpr (more) {
-        load_scales(at(t + 1));
+        copy_scales(~t & 1, at(t + 1));
         a0.copy(smem, nxt, at(t + 1));
       }
       quarter(0, 0);
       if constexpr (!more) GB_WAIT(both ? 2 : 0);
-      else GB_WAIT((both ? 4 : 2) + (TY == GT_FP8 ? 4 : 0));
+      else GB_WAIT((both ? 4 : 2) + (SCALES ? 1 : 0));
       __builtin_amdgcn_s_barrier();
       read_b(cur, 1);
       if constexpr (more) b0.copy(smem, nxt + 2 * HALF, at(t + 1));
@@ -887,7 +880,7 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       quarter(0, 1);
       if constexpr (both) {
         if constexpr (!more) GB_WAIT(0);
-        else GB_WAIT(4 + (TY == GT_FP8 ? 4 : 0));
+        else GB_WAIT(4 + (SCALES ? 1 : 0));
         __builtin_amdgcn_s_barrier();
         read_a(cur, 1);
         if constexpr (more) b1.copy(smem, nxt + 3 * HALF, at(t + 1));
@@ -908,7 +901,7 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       __builtin_amdgcn_s_setprio(1);
     const bool lower = w.m0 + 128 < w.mend;
     auto all = [&](auto both) {
-      load_scales(at(0));
+      copy_scales(0, at(0));
       a0.copy(smem, 0, at(0));
       b0.copy(smem, 2 * HALF, at(0));
       b1.copy(smem, 3 * HALF, at(0));
@@ -935,9 +928,11 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
       a1.template put<false>(smem + HALF, r1, whole, w.kend);
       b0.template put<false>(smem + 2 * HALF, s, whole, w.kend);
       b1.template put<false>(smem + 3 * HALF, s1, whole, w.kend);
-      load_scales(whole);
+      if constexpr (SCALES)
+        *(float*)(smem + 2 * BUF + threadIdx.x * 4) =
+            scale[(long)whole * scale_step];
       __syncthreads();
-      take_scales();
+      read_scales(0);
       read_a(smem, 0);
       read_b(smem, 0);
       quarter(0, 0);

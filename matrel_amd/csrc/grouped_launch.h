@@ -24,7 +24,8 @@ static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
                            : p.T / 256 + p.E + 2;
   auto k = grouped_big_k<TY, AK, BK, WEIGHTS>;
   hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
-                     dim3(512), 2 * 4 * 128 * 128, s, p);
+                     dim3(512),
+                     2 * (4 * 128 * 128 + (TY == GT_FP8 ? 2048 : 0)), s, p);
 }
 
 // Tile codes, as choose_tile (ext_grouped.cpp) picks them.
