@@ -571,8 +571,7 @@ grouped_k(const GroupedArgs p) {
     const bool rows = tid < BM;
     scale = rows ? p.asc + kb * p.T + min(w.m0 + tid, p.T - 1)
                  : p.bsc + ((long)min(w.g, p.E - 1) * ((p.K + 127) / 128) +
-                            kb) * nb +
-                       min(w.n0 / 128 + (tid & (BN / 128 - 1)), nb - 1);
+                            kb) * nb + w.n0 / 128;
     scale_step = rows ? p.T : nb;
   }
 
@@ -587,7 +586,7 @@ grouped_k(const GroupedArgs p) {
       i32x8 y[FM];
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        s[i] = sc[wm + i * 16 + (lane & 15)] * sc[BM + wn / 128];
+        s[i] = sc[wm + i * 16 + (lane & 15)] * sc[BM];
         y[i] = join8(SA::frag(la, wm + i * 16, 0),
                      SA::frag(la, wm + i * 16, 1));
       }
