@@ -73,8 +73,7 @@ __device__ __forceinline__ void put8(unsigned char* o, uint2 q, int have) {
 #define TOP_MIN 0x0d800000u  // 2^-100
 
 // Where rows are not whole lines, neighbouring blocks share lines: they go to
-// one XCD, whose L2 joins them (f32 8 x 2000 x 5000: 94 -> 81 us; bf16 16384 x
-// 8192, whole lines, without / with: 76 / 82 us).
+// one XCD, whose L2 joins them (f32 8 x 2000 x 5000: 94 -> 81 us).
 __device__ __forceinline__ u32 place(long cols) {
   return cols % 128 ? xcd_swizzle(blockIdx.x, gridDim.x) : blockIdx.x;
 }
