@@ -32,6 +32,8 @@ __device__ __forceinline__ i32x4 chunk_at(const typename Elt<TY>::T* row,
   return w;
 }
 
+template <int N> struct Count { static constexpr int n = N; };
+
 // ROWS rows of a K tile, copied to LDS by one wave, 1 KB at a time.
 template <int ROWS> struct WaveSide {
   static constexpr int N = ROWS / 8;
@@ -48,10 +50,11 @@ template <int ROWS> struct WaveSide {
       at[i] = (u32)min(row, last) * ld_bytes + swz(lane & 7, row) * 16;
     }
   }
+  template <int COUNT = N>
   __device__ __forceinline__ void copy(const char* tile, char* lds) const {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < COUNT; ++i)
       glds16(tile + at[i], lds + (i * 64 + lane) * 16);
   }
   static __device__ __forceinline__ i32x4 chunk(const char* lds, int row,
@@ -70,8 +73,7 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
   constexpr int SCALES = TY == GT_FP8 ? 256 : 0;
   constexpr int STAGE = 2048 + 16 * MT * 128 + SCALES;
   constexpr int D = 3;  // 4 and 5 stages a wave measured the same
-  constexpr int OPS = SX::N + SY::N + (SCALES ? 1 : 0);  // copies a stage
-  static_assert((D - 1) * OPS < 64, "counted by vmcnt");
+  static_assert((D - 1) * (SX::N + SY::N + 1) < 64, "counted by vmcnt");
   constexpr int RING = FAST ? W * D * STAGE : 0, SUMS = W * NB * MT * 64 * 16;
   __shared__ __attribute__((aligned(16))) char smem[RING > SUMS ? RING : SUMS];
   f32x4 (*sums)[NB * MT][64] = (f32x4 (*)[NB * MT][64])smem;
@@ -125,7 +127,9 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
       const int all = mine * NB;
       int ci = 0, cslot = 0;
       const char* cx = xb;
-      auto copy = [&]() {
+      // ny: copies of a's rows a stage; up to 8 rows need the first only (what
+      // LDS holds in place of the others makes results that are not stored)
+      auto copy = [&](auto ny) {
         const long tile = wave + (long)ci * W;
         const int slot = cslot;
         cslot = cslot == D - 1 ? 0 : cslot + 1;
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
           glds4(s, lds + 2048 + 16 * MT * 128 + lane * 4);
         }
         sx.copy(cx + tile * 128, lds);
-        sy.copy(yb + tile * 128, lds + 2048);
+        sy.template copy<ny.n>(yb + tile * 128, lds + 2048);
         if (++ci == mine) {
           ci = 0;
           // a block past the end reads the last one again
@@ -171,24 +175,30 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
           }
         }
       };
-      int left = all;  // tiles that are not yet on their way
-      for (int i = 0; i < min(D - 1, all); ++i, --left) copy();
-      int slot = 0;
+      auto run = [&](auto ny) {
+        constexpr int OPS = SX::N + ny.n + (SCALES ? 1 : 0);
+        int left = all;  // tiles that are not yet on their way
+        for (int i = 0; i < min(D - 1, all); ++i, --left) copy(ny);
+        int slot = 0;
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        for (int i = 0; i < mine; ++i) {
-          if (left > 0) {
-            copy();
-            --left;
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * OPS) : "memory");
-          } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int j = 0; j < NB; ++j)
+          for (int i = 0; i < mine; ++i) {
+            if (left > 0) {
+              copy(ny);
+              --left;
+              asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * OPS)
+                           : "memory");
+            } else {
+              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            product(slot, acc[j]);
+            // read to the end, before the slot is copied into
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            slot = slot == D - 1 ? 0 : slot + 1;
           }
-          product(slot, acc[j]);
-          // read to the end, before the slot is copied into
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          slot = slot == D - 1 ? 0 : slot + 1;
-        }
+      };
+      if (MT == 1 && mend - m0 <= 8) run(Count<1>{});
+      else run(Count<SY::N>{});
       first = wave + mine * W;  // at most one tile is left, and ends early
     }
     if (first < tiles)
