@@ -263,8 +263,8 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x);
 
 // c = a @ bt[group]^T of e4m3 operands: a [T, K] with scales [kb][T], or a
 // wider a without scales that is quantized by rows, bt [E, N, K] with scales
-// [E][kb][nb], or one matrix. With `into` (f32, contiguous), the product is written there,
-// or added where `accum` is set.
+// [E][kb][nb], or one matrix. With `into` (f32, contiguous), the product is
+// written there, or added where `accum` is set.
 Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
                         Tensor bsc, c10::optional<Tensor> offs,
                         at::ScalarType out, c10::optional<Tensor> into,

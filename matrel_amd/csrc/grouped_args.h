@@ -1,6 +1,8 @@
 // What the host hands to the grouped products.
 #pragma once
 
+#include <algorithm>
+
 enum GroupedType { GT_BF16 = 0, GT_F16 = 1, GT_F32 = 2, GT_FP8 = 3 };
 
 struct GroupedArgs {
@@ -19,3 +21,9 @@ struct GroupedArgs {
   int out;            // GroupedType of c
   int accum;          // add to c (f32, one split)
 };
+
+// Row tiles of T rows in E groups, a head and a tail, at most: each of these
+// ranges that is not empty can end inside a tile, and no more than T are not.
+inline long grouped_row_tiles(const GroupedArgs& p, int bm) {
+  return p.T / bm + std::min((long)p.E + 2, (long)p.T);
+}

@@ -7,9 +7,8 @@ template <int TY, int BM, int BN, int WM, int WN, int D, bool AK, bool BK,
           bool WEIGHTS, RowsPath PATH>
 static void grouped_go(const GroupedArgs& p, hipStream_t s) {
   const long ntn = (p.N + BN - 1) / BN;
-  // every range of rows that is not empty can end inside one tile more
   const long ntm = WEIGHTS ? (long)p.E * ((p.M + BM - 1) / BM)
-                           : p.T / BM + p.E + 2;
+                           : grouped_row_tiles(p, BM);
   const size_t lds =
       D * ((BM + BN) * 128 + (TY == GT_FP8 ? WM * WN * 256 : 0));
   auto k = grouped_k<TY, BM, BN, WM, WN, D, AK, BK, WEIGHTS, PATH>;
@@ -21,14 +20,14 @@ template <int TY, bool AK, bool BK, bool WEIGHTS>
 static void grouped_big_go(const GroupedArgs& p, hipStream_t s) {
   const long ntn = (p.N + 255) / 256;
   const long ntm = WEIGHTS ? (long)p.E * ((p.M + 255) / 256)
-                           : p.T / 256 + p.E + 2;
+                           : grouped_row_tiles(p, 256);
   auto k = grouped_big_k<TY, AK, BK, WEIGHTS>;
   hipLaunchKernelGGL(k, dim3((unsigned)(ntm * ntn), (unsigned)p.splits),
                      dim3(512),
                      2 * (4 * 128 * 128 + (TY == GT_FP8 ? 2048 : 0)), s, p);
 }
 
-// Tile codes, as choose_tile (ext_grouped.cpp) picks them.
+// Tile codes, as ext_grouped.cpp picks them.
 //   -1, -2: 16, 32 rows, columns by 16 (b with k along its rows)
 //   0: 32 x 128   1: 64 x 64   2: 128 x 128   3: 256 x 256 (not f32)
 // Stages: as many as let two workgroups (64 x 64: three) share a CU's LDS.

@@ -276,7 +276,7 @@ template <int TY, int MT, int NB>
 static void grouped_skinny_nb(const GroupedArgs& p, bool fast, bool eight,
                               hipStream_t s) {
   const long wgs =
-      (p.T / (16 * MT) + p.E + 2L) * ((p.N + 16 * NB - 1) / (16 * NB));
+      grouped_row_tiles(p, 16 * MT) * ((p.N + 16 * NB - 1) / (16 * NB));
 #define GO(W, FAST)                                                         \
   hipLaunchKernelGGL((grouped_skinny_k<TY, MT, NB, W, FAST>),          \
                      dim3((unsigned)wgs), dim3(64 * W), 0, s, p)
