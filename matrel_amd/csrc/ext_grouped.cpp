@@ -94,6 +94,19 @@ struct Plan {
   int tile, splits;
 };
 
+// A launch holds fewer than 2^32 threads. For row tiles of 16 or 32 the grid
+// is counted in blocks of 64 columns, which is what so many get.
+void check_grid(const GroupedArgs& p, int tile, int path, bool weights) {
+  const int bm = tile == -1 ? 16 : tile == -2 || tile == 0 ? 32
+                 : path == 2 || tile == 1 ? 64 : tile == 2 ? 128 : 256;
+  const int bn = tile == 0 ? 128 : std::max(bm, 64);
+  const int64_t rows = weights ? (int64_t)p.E * ((p.M + bm - 1) / bm)
+                               : grouped_row_tiles(p, bm);
+  TORCH_CHECK(rows * ((p.N + bn - 1) / bn) <
+                  (int64_t(1) << 32) / (bm == 256 ? 512 : 256),
+              "product has too many tiles");
+}
+
 // The largest tile whose number fills the chip (codes: grouped_launch.h), and
 // into how many parts long sums are split where even small tiles do not.
 // count(bm, bn): tiles of a size. Measured, us (64 x 64 / 128 x 128 / 256 x
@@ -204,6 +217,7 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
                    : 1;
   const Plan plan = choose_rows(ty, bk, path == 0, T, E, K, N);
   const hipStream_t s = stream_of(a);
+  check_grid(p, plan.tile, path, false);
   const Tensor part = begin(p, c, plan.splits);
   launch_rows(p, ty, plan.tile, bk, path, s);
   finish(p, c, s);
@@ -251,6 +265,7 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   });
   const int tile = plan.tile;
   const hipStream_t s = stream_of(a);
+  check_grid(p, tile, path, true);
   const Tensor part = begin(p, c, plan.splits);
   if (ty == GT_BF16) launch_grouped_bf16(&p, tile, 0, 1, path, s);
   else if (ty == GT_F16) launch_grouped_f16(&p, tile, 0, 1, path, s);
@@ -331,6 +346,7 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
                    : 1;
   const Plan plan = choose_rows(GT_FP8, true, path == 0, T, E, K, N);
   const hipStream_t s = stream_of(a);
+  check_grid(p, plan.tile, path, false);
   const Tensor part = begin(p, c, accum ? 1 : plan.splits);
   launch_rows(p, GT_FP8, plan.tile, true, path, s);
   finish(p, c, s);
@@ -349,7 +365,8 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x) {
   Tensor s = torch::empty({(C + 127) / 128, R},
                           x.options().dtype(torch::kFloat32));
   if (q.numel() == 0) return {q, s};
-  TORCH_CHECK((C + 127) / 128 * ((R + 15) / 16) < (int64_t(1) << 31),
+  // a launch holds fewer than 2^32 threads
+  TORCH_CHECK((C + 127) / 128 * ((R + 15) / 16) < (int64_t(1) << 24),
               "matrix is too large");
   const int64_t ld = R > 1 ? x.stride(0) : 0;
   launch_fp8_quantize_row(x.data_ptr(), ty, ld, R, C, q.data_ptr(),
@@ -381,7 +398,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
     st = torch::empty({0}, of);
   }
   if (q.numel() == 0) return {q, s, qt, st};
-  TORCH_CHECK(rb * cb < (int64_t(1) << 31) && E < 65536,
+  TORCH_CHECK(rb * cb < (int64_t(1) << 24) && E < 65536,
               "matrix is too large");
   const int64_t ld = R > 1 ? x.stride(1) : 0, bld = E > 1 ? x.stride(0) : 0;
   launch_fp8_quantize_tile(x.data_ptr(), ty, ld, bld, E, R, C, q.data_ptr(),

@@ -400,3 +400,13 @@ def test_other_streams():
     assert_near(g, *rows(torch.ones(70, 320, dtype=torch.float64,
                                     device="cuda"),
                          w.double().transpose(1, 2).contiguous(), off), 320)
+
+
+def test_refuses_more_tiles_than_a_launch_holds():
+    """As many groups as rows: a tile for every row, 2^32 threads and more."""
+    t, k, n = 1 << 17, 16, 8192
+    a = torch.zeros(t, k, dtype=BF, device="cuda")
+    b = torch.zeros(1, n, k, dtype=BF, device="cuda").expand(t, n, k)
+    off = torch.arange(t + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        ma.grouped_matmul(a, b.transpose(1, 2), off)
