@@ -107,32 +107,49 @@ void check_grid(const GroupedArgs& p, int tile, int path, bool weights) {
               "product has too many tiles");
 }
 
-// The largest tile whose number fills the chip (codes: grouped_launch.h), and
-// into how many parts long sums are split where even small tiles do not.
-// count(bm, bn): tiles of a size. Measured, us (64 x 64 / 128 x 128 / 256 x
-// 256; the rule counts 128 x 128 tiles):
-//   bf16 4096 rows, 12 groups, 1024 x 1000 (352): 34 / 26 / 31
-//   bf16 300 rows, 4 groups, 2048 x 1024 (96): 9 / 17 / 25
-//   fp8 5003 rows, 24 groups, 1536 x 2560 (756): 66 / 68 / 46
-//   f32 4096 rows, 12 groups, 1024 x 1000 (352): 106 / 138 / -
-//   fp16 unaligned, 3001 rows, 10 groups, 1111 x 777, d_b (630): 36 / 50 / -
+// Into how many parts long sums are split where even small tiles do not fill
+// the chip.
 int choose_splits(int64_t tiles, int64_t k_tiles) {
   // the join is a launch and a pass over the parts: not for short sums
   if (tiles >= 192 || k_tiles < 16) return 1;
   return (int)std::min<int64_t>({k_tiles / 4, (383 + tiles) / tiles, 16});
 }
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles (codes: grouped_launch.h). Measured, us, 64 x 64 / 128 x 128 / 256 x
+// 256, behind the number of 256 x 256 ones that the host counts:
+//   rows, bf16 8192 rows, 8 groups, 1112 x 776 (190): 39 / 36 / 27
+//   rows, bf16 8192 rows, 32 groups, 1536 x 1032 (280): 57 / 48 / 71
+//   rows, fp8 16384 rows, 8192 x 8192 (2048): the large one 1.2 x the middle
+//   rows, bf16 913 rows, 24 groups, 1344 x 2904: 39 / 44 / 64
+//   d_b, bf16 8192 rows, 32 groups, 1536 x 1032 (960): 109 / 71 / 62
+//   d_b, bf16 8192 rows, 8 groups, 2048 x 2048 (512): 123 / 84 / 104
+//   d_b, bf16 8192 rows, 8 groups, 1112 x 776 (160): 42 / 61 / 97
+//   d_b, bf16 10641 rows, 3 groups, 2232 x 1632 (189): 158 / 104 / 87
+//   rows, f32 4096 rows, 12 groups, 1024 x 1000: 106 / 138 / -
+//   d_b, fp16 unaligned, 3001 rows, 10 groups, 1111 x 777: 36 / 50 / -
+// Over 38 other shapes drawn at random the choice takes 1.02 - 1.05 of the
+// best tile's time on average.
+
+// Whether 256 x 256 tiles take less time in rounds over the chip's 256 CUs,
+// one on each, than 128 x 128 ones, two on each: a round of large tiles takes
+// 3/2 of the time of one of small ones, which are half as much work.
+bool large_pays(int64_t large, int64_t middle) {
+  return 3 * ceil_div(large, 256) <= 2 * ceil_div(middle, 512);
+}
+
+// large: whether 256 x 256 tiles pay; enough: 128 x 128 tiles that do.
 template <class F>
-Plan choose(int ty, bool fast, int64_t k_tiles, F count) {
+Plan choose(int ty, bool fast, bool large, int64_t enough, int64_t k_tiles,
+            F count) {
   Plan p = {1, 1};
-  const int64_t middle = count(128, 128);
-  if (fast && ty != GT_F32 && count(256, 256) >= 200) p.tile = 3;
-  else if (middle >= (fast && ty != GT_F32 ? 250 : 1024)) p.tile = 2;
+  const bool free = fast && ty != GT_F32;
+  if (free && large) p.tile = 3;
+  else if (count(128, 128) >= (free ? enough : 1024)) p.tile = 2;
   if (p.tile == 1) p.splits = choose_splits(count(64, 64), k_tiles);
   return p;
 }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tiles of the rows of E groups, each of which can end inside a tile.
 int64_t row_tiles(int64_t T, int64_t E, int64_t bm) {
@@ -147,9 +164,17 @@ Plan choose_rows(int ty, bool bk, bool fast, int64_t T, int64_t E, int64_t K,
   if (bk && each <= 32) return {each <= 16 ? -1 : -2, 1};
   if (fast && each <= 32)
     return {0, choose_splits(row_tiles(T, E, 32) * ceil_div(N, 128), k_tiles)};
-  return choose(ty, fast, k_tiles, [&](int64_t bm, int64_t bn) {
-    return row_tiles(T, E, bm) * ceil_div(N, bn);
-  });
+  // a group ends inside a tile by half of it on average, short ones by more
+  const auto met = [&](int64_t b) {
+    return (E == 1 ? ceil_div(T, b) : T / b + std::min(E, T) * 3 / 4) *
+           ceil_div(N, b);
+  };
+  // and where all are short, a large tile is mostly empty
+  const bool large = each >= 128 && large_pays(met(256), met(128));
+  return choose(ty, fast, large, 250, k_tiles,
+                [&](int64_t bm, int64_t bn) {
+                  return row_tiles(T, E, bm) * ceil_div(N, bn);
+                });
 }
 
 // Where the kernel writes: c, or partial sums that finish() joins.
@@ -260,9 +285,17 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
                            M % epc == 0 && N % epc == 0 ? 0
                    : 1;
   const int64_t k_tiles = T / E / (ty == GT_F32 ? 32 : 64);
-  const Plan plan = choose(ty, path == 0, k_tiles, [&](int64_t bm, int64_t bn) {
+  const auto count = [&](int64_t bm, int64_t bn) {
     return E * ceil_div(M, bm) * ceil_div(N, bn);
-  });
+  };
+  // the sums of several groups have uneven lengths, which many tiles even out,
+  // unless they are short beside the writing of the results
+  const bool even = E <= 4 || T / E <= 128;
+  const Plan plan =
+      choose(ty, path == 0,
+             even ? large_pays(count(256, 256), count(128, 128))
+                  : count(256, 256) >= 800,
+             even ? 250 : 640, k_tiles, count);
   const int tile = plan.tile;
   const hipStream_t s = stream_of(a);
   check_grid(p, tile, path, true);
