@@ -280,9 +280,13 @@ static void grouped_skinny_nb(const GroupedArgs& p, bool fast, bool eight,
 #define GO(W, FAST)                                                         \
   hipLaunchKernelGGL((grouped_skinny_k<TY, MT, NB, W, FAST>),          \
                      dim3((unsigned)wgs), dim3(64 * W), 0, s, p)
-  if (fast && eight) GO(8, true);
-  else if (fast) GO(4, true);
-  else if (eight) GO(8, false);
+  if constexpr (NB == 1)
+    if (eight) {
+      if (fast) GO(8, true);
+      else GO(8, false);
+      return;
+    }
+  if (fast) GO(4, true);
   else GO(4, false);
 #undef GO
 }

@@ -2,13 +2,15 @@
 engine's fp8 tier, graphs, streams and large tensors.
 
 References are float64 products on the GPU. Tolerances as in
-test_grouped_fp8.py: (K + 8) * 2^-23 * sum |a b| for a float32 sum, half a
-step of the result's type for its rounding."""
+test_grouped_fp8.py: (K + 8) * 2^-23 * sum |a b| for a float32 sum, what the
+8-bit matrix unit cuts off (fp8_cut), half a step of the result's type for its
+rounding."""
 
 import pytest
 import torch
 
 import matrel_amd as ma
+from test_grouped_fp8 import fp8_cut
 
 pytestmark = pytest.mark.gpu
 
@@ -28,8 +30,10 @@ def offsets_of(sizes, head=0):
     return torch.tensor(v, dtype=torch.int32, device="cuda")
 
 
-def assert_near(got, exact, size, depth):
-    err = (depth + 8) * 2.0 ** -23 * size
+def assert_near(got, exact, size, depth, cut=0.0):
+    if torch.is_tensor(cut):
+        cut = cut.to(size.device)
+    err = (depth + 8) * 2.0 ** -23 * size + cut
     tol = err + torch.finfo(got.dtype).eps / 2 * (exact.abs() + err)
     if got.dtype == HF:
         tol = tol + 2.0 ** -25
@@ -140,14 +144,60 @@ def test_fp8_tiles(sizes, k, n, dtype):
         return q.data.double() * s
 
     assert_near(y, *rows(values(qa), values(qw).transpose(1, 2).contiguous(),
-                         off), k + 128)
-    assert_near(da, *rows(values(qg), values(qw), off), n + 128)
+                         off), k, fp8_cut(qa, qw, off))
+    assert_near(da, *rows(values(qg), values(qw), off), n,
+                fp8_cut(qg, qw.transpose(), off))
     v, ad, gd = off.tolist(), a.detach().double(), gy.double()
     for g, (lo, hi) in enumerate(zip(v, v[1:])):
         x, z = gd[lo:hi], ad[lo:hi]
         assert_near(dw[g], x.t() @ z, x.abs().t() @ z.abs(), hi - lo)
     assert torch.equal(y, ma.fp8_matmul(a, w, off))
     assert torch.equal(y, ma.fp8_matmul(qa, qw, off, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("sizes,k,n", [
+    ([1300, 1, 1299], 200, 4104),    # the product
+    ([1300, 0, 1300], 4104, 200),    # the gradient of a
+    ([130, 1, 70], 1032, 3080),      # the gradient of b, few groups
+    ([300] * 32, 1032, 1544),        # the same, many
+])
+def test_large_tile(sizes, k, n, dtype, layout):
+    """256 x 256, with ends of groups, columns and sums inside a tile."""
+    check_grouped(sizes, k, n, dtype, layout)
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [HF, FF])
+@pytest.mark.parametrize("sizes,k,n", [
+    ([2000, 1, 2099], 17, 4099),     # the product
+    ([33, 7, 60], 2305, 1545),       # the gradient of b
+])
+def test_middle_tile_unaligned(sizes, k, n, dtype, layout):
+    check_grouped(sizes, k, n, dtype, layout)
+
+
+FEW = [([3] * 20, 6400), ([3, 3], 6400), ([3], 1000),      # 16 rows: 4, 2, 1
+       ([20] * 20, 6400), ([20, 40], 5000), ([20], 1000)]  # 32 rows
+
+
+@pytest.mark.parametrize("k", [136, 137, 4096, 4099])
+@pytest.mark.parametrize("dtype", [BF, HF, FF])
+@pytest.mark.parametrize("sizes,n", FEW)
+def test_few_rows(sizes, n, k, dtype):
+    """Blocks of columns a workgroup, four waves or (long sums) eight."""
+    if k < 4096 or n == 1000:
+        check_grouped(sizes, k, n, dtype, "nk")
+
+
+@pytest.mark.parametrize("sizes,k,n", [
+    ([1300, 1, 1299], 208, 4104), ([2000, 1, 2099], 131, 4099),  # large tiles
+    ([100, 100], 7, 40)] +                                 # rows of a few bytes
+    [(s, k, n) for s, n in FEW for k in (144, 145)] +
+    [(s, k, 1000) for s, n in FEW if n == 1000 for k in (8192, 8195)])
+def test_fp8_variants(sizes, k, n):
+    test_fp8_tiles(sizes, k, n, BF)
 
 
 def test_far_rows():
@@ -202,11 +252,13 @@ def test_engine_fp8_tier():
         ta, tb = randn(700, 900, seed=15), randn(900, 650, seed=16)
         c = (s.from_dense(ta) @ s.from_dense(tb)).to_tensor()
         # 512 is a multiple of 128: blocks quantize as the whole does
-        qa = ma.quantize_fp8(ta).dequantize().double()
-        qb = ma.quantize_fp8(tb.t(), "tile").dequantize().double().t()
+        fa, fb = ma.quantize_fp8(ta), ma.quantize_fp8(tb.t()[None], "tile")
+        qa = fa.dequantize().double()
+        qb = fb.dequantize()[0].double().t()
         assert c.shape == (700, 650)
         assert torch.equal(c, c.to(BF).float())  # as the engine stores it
-        assert_near(c.to(BF), qa @ qb, qa.abs() @ qb.abs(), 900 + 256)
+        assert_near(c.to(BF), qa @ qb, qa.abs() @ qb.abs(), 900,
+                    fp8_cut(fa, fb, offsets_of([700])))
     finally:
         ma.set_config(old)
         reset_runtime()
@@ -258,9 +310,10 @@ def test_block_accumulate():
     one = acc.clone()
     blockops.gemm_bt_fp8_acc(acc, qa, sa, qb, sb)
     assert torch.equal(acc, 2 * one)
-    x = ma.quantize_fp8(a).dequantize().double()
-    y = ma.quantize_fp8(bt, "tile").dequantize().double()
-    assert_near(one, x @ y.t(), x.abs() @ y.abs().t(), 260 + 128)
+    fa, fb = ma.quantize_fp8(a), ma.quantize_fp8(bt[None], "tile")
+    x, y = fa.dequantize().double(), fb.dequantize()[0].double()
+    assert_near(one, x @ y.t(), x.abs() @ y.abs().t(), 260,
+                fp8_cut(fa, fb, offsets_of([130])))
 
 
 def serve(x, w1, w2, off):
