@@ -293,7 +293,7 @@ static void grouped_skinny_nb(const GroupedArgs& p, bool fast, bool eight,
 
 // Blocks of 16 columns a workgroup, by how many blocks there are: a workgroup
 // costs about 2 us beside its reading, but the chip has to be filled. bf16,
-// 64 rows in 8 groups of 4096 x 4096 (3072 blocks by this count), 1 / 2 / 4
+// 64 rows in 8 groups of 4096 x 4096 (12 x 256 by this count), 1 / 2 / 4
 // blocks: 73 / 52 / 61 us; one row, 4096 x 4096 (256): 8.5 / 11.1 / 15.3 us;
 // fp8, 64 rows in 32 groups of 4096 x 2048 (9216): 43 / 34 / 31 us. With few
 // blocks and a long sum, eight waves share it instead of four.
