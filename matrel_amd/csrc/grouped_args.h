@@ -27,3 +27,16 @@ struct GroupedArgs {
 inline long grouped_row_tiles(const GroupedArgs& p, int bm) {
   return p.T / bm + std::min((long)p.E + 2, (long)p.T);
 }
+
+// Few rows: a workgroup makes blocks of 16 columns from n0 on, one after
+// another. The first column of block j; where fewer blocks are left, of the
+// last one that holds a column.
+constexpr int few_rows_block(int n, int n0, int j) {
+  return n0 + 16 * std::min(j, (n - 1 - n0) / 16);
+}
+
+// Row i of the 16 rows of b that such a block reads, from its first one: a
+// block that ends early reads its last row again.
+constexpr int few_rows_row(int n, int block, int i) {
+  return std::min(i, n - 1 - block);
+}

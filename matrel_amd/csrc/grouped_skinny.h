@@ -114,18 +114,17 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
     if constexpr (FAST) {
       SX sx;
       SY sy;
-      sx.init((u32)p.ldb * ES, p.N - 1 - n0);
+      sx.init((u32)p.ldb * ES, few_rows_row(p.N, n0, 15));
       sy.init((u32)p.lda * ES, mend - 1 - m0);
       const char* xb = (const char*)((const E*)p.b + (long)g * p.gsb +
                                      (long)n0 * p.ldb);
       const char* yb = (const char*)((const E*)p.a + (long)m0 * p.lda);
-      const long xstep = 16L * p.ldb * ES;
       char* ring = smem + wave * (D * STAGE);
       const int whole = p.K / BKE;
       const int mine = whole > wave ? (whole - wave + W - 1) / W : 0;
       // the ring runs on over the NB blocks of 16 columns
       const int all = mine * NB;
-      int ci = 0, cslot = 0;
+      int ci = 0, cslot = 0, cblock = 0;
       const char* cx = xb;
       // ny: copies of a's rows a stage; up to 8 rows need the first only (what
       // LDS holds in place of the others makes results that are not stored)
@@ -144,8 +143,11 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
         sy.template copy<ny.n>(yb + tile * 128, lds + 2048);
         if (++ci == mine) {
           ci = 0;
-          // a block past the end reads the last one again
-          if (n0 + (int)((cx - xb) / xstep + 1) * 16 < p.N) cx += xstep;
+          if constexpr (NB > 1) {  // the next block, which can end earlier
+            const int at = few_rows_block(p.N, n0, ++cblock);
+            cx = xb + (long)(at - n0) * p.ldb * ES;
+            sx.init((u32)p.ldb * ES, few_rows_row(p.N, at, 15));
+          }
         }
       };
       auto product = [&](int slot, f32x4 (&acc)[MT]) {

@@ -1,0 +1,73 @@
+"""Grouped and 8-bit products where operands, sizes and modes end: column
+blocks past the last column, captures beside eager graphs, forward mode,
+scales and gradients near the ends of a type's range.
+
+Tolerances as in test_grouped_fp8.py."""
+
+import os
+import subprocess
+
+import pytest
+import torch
+
+import matrel_amd as ma
+from test_grouped_fp8 import (DEVICES, assert_near, fp8_cut, offsets_of,
+                              plain_rows, plain_weights, randn, values_of)
+
+CSRC = os.path.join(os.path.dirname(os.path.abspath(ma.__file__)), "csrc")
+
+# Every row of b that the few-rows kernel's ring reads: block j of the NB of a
+# workgroup, its 16 rows, for all workgroups of n columns.
+FEW_ROWS = r"""
+#include "grouped_args.h"
+#include <cstdio>
+int main() {
+  for (int nb : {1, 2, 4})
+    for (int n = 1; n <= 300; ++n)
+      for (int n0 = 0; n0 < n; n0 += 16 * nb)
+        for (int j = 0; j <= nb; ++j)  // the ring steps on once too often
+          for (int i = 0; i < 16; ++i) {
+            const int block = few_rows_block(n, n0, j);
+            const int last = few_rows_row(n, block, 15);
+            const int row = block + (i < last ? i : last);
+            const int want = n0 + j * 16 + i;
+            if (row < 0 || row >= n || row != block + few_rows_row(n, block, i)
+                || (want < n && j < nb && row != want)) {
+              std::printf("nb %d n %d n0 %d block %d row %d reads %d\n", nb, n,
+                          n0, j, i, row);
+              return 1;
+            }
+          }
+}
+"""
+
+
+def test_few_rows_reads_rows_that_exist(tmp_path):
+    src, exe = tmp_path / "few.cpp", tmp_path / "few"
+    src.write_text(FEW_ROWS)
+    subprocess.run(["g++", "-std=c++17", "-I", CSRC, str(src), "-o",
+                    str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16,
+                                   torch.float32])
+@pytest.mark.parametrize("sizes,k,n", [
+    ([1] * 64, 256, 1400),       # 16 rows, two blocks, 24 columns left
+    ([3] * 16, 256, 4120),       # the same, 24 left
+    ([2] * 140, 128, 1000),      # four blocks, 40 left
+    ([20] * 12, 256, 1400),      # 32 rows, two blocks
+    ([20] * 140, 128, 1000)])    # 32 rows, four blocks
+def test_few_rows_last_columns(sizes, k, n, dtype):
+    """Column blocks that end early behind others of their workgroup."""
+    off = offsets_of(sizes, "cuda")
+    a = randn(sum(sizes), k, seed=1, dtype=dtype, device="cuda")
+    w = randn(len(sizes), n, k, seed=2, dtype=dtype, device="cuda")
+    b = w.transpose(1, 2)
+    assert_near(ma.grouped_matmul(a, b, off), *plain_rows(a, b, off), k)
+    qa, qw = ma.quantize_fp8(a), ma.quantize_fp8(w, "tile")
+    assert_near(ma.fp8_matmul(qa, qw, off, out_dtype=dtype),
+                *plain_rows(values_of(qa), values_of(qw).transpose(1, 2), off),
+                k, fp8_cut(qa, qw, off))
