@@ -24,7 +24,8 @@ import torch
 
 from .backend import require_ext, use_hip
 from .grouped import (check_capture, check_offsets, check_out_dtype,
-                      needs_grad, rows_product, weights_product)
+                      needs_grad, refuse_tangents, rows_product,
+                      weights_product)
 
 BLOCK = 128
 _MAX = 448.0
@@ -243,6 +244,7 @@ def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
         check_offsets(offsets, bt.shape[0], a.shape[0], a.device)
     out_dtype = check_out_dtype(
         out_dtype, torch.bfloat16 if isinstance(a, Fp8Blocks) else a.dtype)
+    refuse_tangents(*(t for t in (a, bt) if isinstance(t, torch.Tensor)))
     if isinstance(a, Fp8Blocks):
         if isinstance(bt, torch.Tensor):
             if bt.requires_grad and torch.is_grad_enabled():

@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .backend import require_ext, use_hip
 
@@ -55,6 +56,16 @@ def check_out_dtype(out_dtype: Optional[torch.dtype],
 
 def needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def refuse_tangents(*tensors) -> None:
+    """Forward-mode tangents, which requires_grad does not show: the kernels
+    carry none, and a result without one would count as constant."""
+    if forward_ad._current_level < 0:
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("grouped and 8-bit products have no "
+                                  "forward-mode derivative")
 
 
 def check_capture(*leaves) -> None:
@@ -133,6 +144,8 @@ def grouped_matmul_grads(grad: torch.Tensor, a: torch.Tensor,
         raise ValueError(f"grad must be {(a.shape[0], b.shape[2])} on "
                          f"{a.device}, got {tuple(grad.shape)} on "
                          f"{grad.device}")
+    if use_hip(a):
+        refuse_tangents(grad, a, b)
     with torch.no_grad():
         grad = grad.to(a.dtype)
         return (_grad_a(grad, b, offsets), _grad_b(grad, a, b, offsets))
@@ -183,6 +196,8 @@ def grouped_matmul(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     in a and b."""
     _check(a, b, offsets)
     out_dtype = check_out_dtype(out_dtype, a.dtype)
+    if use_hip(a):
+        refuse_tangents(a, b)
     if not needs_grad(a, b):
         return rows_product(a, b, offsets, out_dtype)
     if not use_hip(a):

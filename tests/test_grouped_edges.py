@@ -9,6 +9,7 @@ import subprocess
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import matrel_amd as ma
 from test_grouped_fp8 import (DEVICES, assert_near, fp8_cut, offsets_of,
@@ -71,3 +72,52 @@ def test_few_rows_last_columns(sizes, k, n, dtype):
     assert_near(ma.fp8_matmul(qa, qw, off, out_dtype=dtype),
                 *plain_rows(values_of(qa), values_of(qw).transpose(1, 2), off),
                 k, fp8_cut(qa, qw, off))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode(device):
+    """A tangent is carried in full or refused, never dropped."""
+    off = offsets_of([3, 5], device)
+    a = randn(8, 136, seed=3, device=device)
+    w = randn(2, 24, 136, seed=4, device=device)
+    ta, tw = randn(8, 136, seed=5, device=device), \
+        randn(2, 24, 136, seed=6, device=device)
+    gy = randn(8, 24, seed=7, device=device)
+    qa, qw = ma.quantize_fp8(a), ma.quantize_fp8(w, "tile")
+    with fwd.dual_level():
+        da, dw = fwd.make_dual(a, ta), fwd.make_dual(w, tw)
+        # with and without a backward pass beside it
+        for x in (da, fwd.make_dual(a.clone().requires_grad_(), ta)):
+            for f in (lambda: ma.fp8_matmul(x, w, off),
+                      lambda: ma.fp8_matmul(x, qw, off)):
+                with pytest.raises(NotImplementedError):
+                    f()
+        for f in (lambda: ma.fp8_matmul(a, dw, off),
+                  lambda: ma.fp8_matmul(qa, dw, off)):
+            with pytest.raises(NotImplementedError):
+                f()
+        b = w.transpose(1, 2)
+        calls = ((da, b), (a, dw.transpose(1, 2)), (da, dw.transpose(1, 2)))
+        for x, y in calls:
+            if device == "cuda":
+                with pytest.raises(NotImplementedError):
+                    ma.grouped_matmul(x, y, off)
+                with pytest.raises(NotImplementedError):
+                    ma.grouped_matmul_grads(gy, x, y, off)
+                continue
+            got = fwd.unpack_dual(ma.grouped_matmul(x, y, off)).tangent
+            want = torch.zeros(8, 24, dtype=torch.float64)
+            size = torch.zeros_like(want)
+            if x is da:
+                p = plain_rows(ta, b, off)
+                want, size = want + p[0], size + p[1]
+            if y is not b:
+                p = plain_rows(a, tw.transpose(1, 2), off)
+                want, size = want + p[0], size + p[1]
+            assert_near(got, want, size, 2 * 136)
+        # no tangent: as ever, also inside of a level
+        assert torch.equal(ma.fp8_matmul(a, w, off),
+                           ma.fp8_matmul(qa, qw, off, torch.float32))
+        assert fwd.unpack_dual(ma.grouped_matmul(a, b, off)).tangent is None
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: ma.fp8_matmul(x, w, off), (a,), (ta,))
