@@ -11,6 +11,8 @@
 
 #include <algorithm>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "grouped_args.h"
 
@@ -570,15 +572,45 @@ Tensor fp8_matmul(Tensor a, c10::optional<Tensor> w, c10::optional<Tensor> q,
   return Fp8Matmul::apply(a, w, q, s, offs, (int64_t)out);
 }
 
-// Whether an autograd graph that met this leaf on another stream than the
-// current one still lives.
+// Whether the current stream of t's device is being captured.
+bool capturing(const Tensor& t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  const hipError_t e = hipStreamIsCapturing(stream_of(t), &status);
+  TORCH_CHECK(e == hipSuccess, "HIP error: ", hipGetErrorString(e));
+  return status != hipStreamCaptureStatusNone;
+}
+
+// Whether the backward pass behind t, a leaf or not, would run nodes on a
+// stream that is neither the current one nor captured with it: those of a
+// leaf that an autograd graph from there still holds, or of what was computed
+// there.
 bool held_by_other_stream(const Tensor& t) {
-  if (!t.requires_grad() || !t.is_leaf()) return false;
-  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!held || held->num_inputs() == 0) return false;
-  // by id: the one is of device type "cuda", the other "hip"
-  return held->input_metadata(0).stream().id() !=
-         c10::hip::getCurrentHIPStream(t.device().index()).id();
+  using torch::autograd::Node;
+  if (!t.requires_grad()) return false;
+  std::vector<std::shared_ptr<Node>> left = {
+      t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t)
+                  : t.grad_fn()};
+  std::unordered_set<Node*> met;
+  while (!left.empty()) {
+    const std::shared_ptr<Node> node = std::move(left.back());
+    left.pop_back();
+    if (!node || !met.insert(node.get()).second) continue;
+    if (const auto s = node->stream()) {
+      // by id: the one is of device type "cuda", the other "hip"
+      if (s->id() != c10::hip::getCurrentHIPStream(s->device_index()).id()) {
+        // the default stream (0) is never captured
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (s->id() == 0 ||
+            hipStreamIsCapturing(
+                c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s)
+                    .stream(), &status) != hipSuccess ||
+            status == hipStreamCaptureStatusNone)
+          return true;
+      }
+    }
+    for (const auto& edge : node->next_edges()) left.push_back(edge.function);
+  }
+  return false;
 }
 
 }  // namespace
@@ -596,5 +628,8 @@ void bind_grouped(pybind11::module& m) {
         "e4m3 with a scale for each 128 x 128 tile");
   m.def("grouped_matmul", &grouped_matmul, "differentiable grouped_rows");
   m.def("fp8_matmul", &fp8_matmul, "differentiable grouped_rows_fp8");
-  m.def("held_by_other_stream", &held_by_other_stream);
+  m.def("capturing", &capturing,
+        "whether the current stream of a tensor's device is captured");
+  m.def("held_by_other_stream", &held_by_other_stream,
+        "whether a tensor's backward pass would run on another stream");
 }

@@ -68,15 +68,16 @@ def refuse_tangents(*tensors) -> None:
                                   "forward-mode derivative")
 
 
-def check_capture(*leaves) -> None:
-    """Autograd runs a leaf's accumulation on the stream of the graph that
-    met it first. A backward pass captured while such an outside graph lives
-    would make the capture wait for that stream, which ends the process: it
-    is refused here, before anything is recorded."""
-    if not leaves[0].is_cuda \
-            or not torch.cuda.is_current_stream_capturing():
+def check_capture(*operands) -> None:
+    """Autograd runs a node of a backward pass on the stream of its forward
+    pass, and a leaf's accumulation on the stream of the graph that met it
+    first. A backward pass captured while an operand or a leaf behind it (a
+    view's, say) has nodes outside would make the capture wait for that
+    stream, which ends the process: it is refused here, before anything is
+    recorded."""
+    if not operands[0].is_cuda or not require_ext().capturing(operands[0]):
         return
-    for t in leaves:
+    for t in operands:
         if require_ext().held_by_other_stream(t):
             raise RuntimeError(
                 "an autograd graph built outside of this capture still "

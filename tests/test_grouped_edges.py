@@ -121,3 +121,73 @@ def test_forward_mode(device):
         assert fwd.unpack_dual(ma.grouped_matmul(a, b, off)).tangent is None
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: ma.fp8_matmul(x, w, off), (a,), (ta,))
+
+
+@pytest.mark.gpu
+def test_capture_guard_sees_through_views():
+    """What a graph of another stream holds, behind views and casts too."""
+    from matrel_amd.ops.backend import require_ext
+    held = require_ext().held_by_other_stream
+    w = randn(2, 64, 64, seed=8, device="cuda").requires_grad_()
+    x = randn(9, 64, seed=9, device="cuda").requires_grad_()
+    forms = (lambda: w, lambda: w.transpose(1, 2),
+             lambda: w.to(torch.bfloat16), lambda: (w * 2)[:, :8],
+             lambda: w[0].expand(3, 64, 64))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    assert not any(held(f()) for f in forms)
+    with torch.cuda.stream(side):  # no graph lives: nothing is held
+        assert not any(held(f()) for f in forms)
+        assert not held(w.detach()) and not held(torch.ones(3, device="cuda"))
+    torch.cuda.synchronize()
+    alive = w * 1
+    outside = x * 1
+    assert not any(held(f()) for f in forms)
+    with torch.cuda.stream(side):
+        assert all(held(f()) for f in forms)
+        assert held(outside) and held(outside[:4]) and not held(w.detach())
+    del alive, outside
+    with torch.cuda.stream(side):
+        assert not any(held(f()) for f in forms) and not held(x)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_living_graph_of_a_view():
+    """A captured forward pass is refused for views of held leaves and for
+    operands that were computed outside, and for nothing else."""
+    bf = dict(dtype=torch.bfloat16, device="cuda")
+    a = randn(64, 64, seed=10, **bf)
+    w = randn(2, 64, 64, seed=11, **bf).requires_grad_()
+    free = randn(2, 64, 64, seed=12, **bf).requires_grad_()
+    off = offsets_of([30, 34], "cuda")
+    alive = ma.grouped_matmul(a, w.transpose(1, 2), off)
+    outside = randn(64, 64, seed=13, **bf).requires_grad_() * 2
+    want = ma.grouped_matmul(a, free.transpose(1, 2), off).detach()
+    torch.cuda.synchronize()
+    refused, taken = 0, []
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in (lambda: ma.grouped_matmul(a, w.transpose(1, 2), off),
+                  lambda: ma.fp8_matmul(a, w.reshape(2, 64, 64), off),
+                  lambda: ma.grouped_matmul(outside, free, off),
+                  lambda: ma.fp8_matmul(outside, free, off)):
+            try:
+                f()
+            except RuntimeError as e:
+                refused += "outside of this capture" in str(e)
+        taken.append(ma.grouped_matmul(a, free.transpose(1, 2), off))
+        taken.append(ma.grouped_matmul(a, w.detach().transpose(1, 2), off))
+        # a stream that the capture itself forks is inside
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            forked = free.transpose(1, 2) * 1
+        torch.cuda.current_stream().wait_stream(side)
+        taken.append(ma.grouped_matmul(a, forked, off))
+    assert refused == 4 and len(taken) == 3
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(taken[0], want) and torch.equal(taken[2], want)
+        assert torch.equal(taken[1], alive)
