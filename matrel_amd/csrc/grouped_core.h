@@ -527,6 +527,52 @@ template <bool WEIGHTS> struct Results {
   }
 };
 
+// ---- scales whose product overflows -----------------------------------------
+
+// Zero where all four are finite, else NaN.
+__device__ __forceinline__ float zero4(f32x4 v) {
+  return (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+}
+
+// fp8: a lane's four sums over [kbeg, kend) at (row, col). A block pair whose
+// scales are finite and their product is not makes infinities, or NaN of a
+// payload sum of 0, where the values' own products can be finite. Such sums
+// are taken again, one value at a time, each scaled before it is multiplied.
+// Where all results are finite this costs two operations each.
+__device__ __forceinline__ f32x4 fp8_again(const GroupedArgs& p, int g,
+                                           int row, int col, int kbeg,
+                                           int kend, f32x4 v) {
+  const int nb = (p.N + 127) / 128, kbs = (p.K + 127) / 128;
+  const float* xs = p.asc + row;
+  const float* ys = p.bsc + (long)g * kbs * nb + col / 128;
+  bool over = false;
+#pragma unroll 1
+  for (int kb = kbeg / 128; kb * 128 < kend; ++kb) {
+    const float x = xs[(long)kb * p.T], y = ys[(long)kb * nb];
+    if (x - x != 0 || y - y != 0) return v;  // not a number by its values
+    over |= x * y - x * y != 0;
+  }
+  if (!over) return v;
+  const unsigned char* a = (const unsigned char*)p.a + (long)row * p.lda;
+  const unsigned char* b = (const unsigned char*)p.b + (long)g * p.gsb;
+  f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int k = kbeg; k < kend; ++k) {
+    const float x = __builtin_amdgcn_cvt_f32_fp8(a[k], 0) *
+                    xs[(long)(k / 128) * p.T];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = min(col + q, p.N - 1);
+      const float y = __builtin_amdgcn_cvt_f32_fp8(b[(long)n * p.ldb + k], 0) *
+                      ys[(long)(k / 128) * nb];
+      sum[q] = __builtin_fmaf(x, y, sum[q]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = v[q] - v[q] == 0 ? v[q] : sum[q];
+  return v;
+}
+
 // ---- small and middle tiles ------------------------------------------------
 
 // BM x BN results a workgroup, its waves WM x WN. AK/BK: the operand has k
@@ -715,6 +761,22 @@ grouped_k(const GroupedArgs p) {
   }
 
   const Results<WEIGHTS> out(p, w);
+  if constexpr (TY == GT_FP8) {
+    float z = 0;
+#pragma unroll
+    for (int i = 0; i < FM * FN; ++i) z += zero4(((f32x4*)acc)[i]);
+    if (z != 0) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int row = w.m0 + wm + i * 16 + (lane & 15);
+          const int col = w.n0 + wn + j * 16 + (lane >> 4) * 4;
+          if (row < w.mend && col < p.N && zero4(acc[j][i]) != 0)
+            acc[j][i] = fp8_again(p, w.g, row, col, w.kbeg, w.kend, acc[j][i]);
+        }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -952,6 +1014,22 @@ __global__ void __launch_bounds__(512) grouped_big_k(const GroupedArgs p) {
     __builtin_amdgcn_s_setprio(0);
   }
 
+  if constexpr (TY == GT_FP8) {
+    float z = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z += zero4(((f32x4*)acc)[i]);
+    if (z != 0) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        f32x4& v = ((f32x4*)acc)[i];
+        const int row = w.m0 + (i >> 4) * 128 + qr + (i & 1) * 16 + (lane & 15);
+        const int col = w.n0 + (i >> 3 & 1) * 128 + qc + (i >> 1 & 3) * 16 +
+                        (lane >> 4) * 4;
+        if (row < w.mend && col < p.N && zero4(v) != 0)
+          v = fp8_again(p, w.g, row, col, w.kbeg, w.kend, v);
+      }
+    }
+  }
   const Results<WEIGHTS> out(p, w);
   if (out.ty != GT_F32 && out.n % 8 == 0 && (u64)out.c % 16 == 0) {
     // 16-bit results turn round in LDS, so that 32 lanes store 512 bytes of

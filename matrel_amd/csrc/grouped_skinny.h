@@ -264,6 +264,8 @@ __global__ void __launch_bounds__(64 * W) grouped_skinny_k(const GroupedArgs p) 
     for (int i = 1; i < W; ++i) sum += sums[i][f][lane];
     const int at = m0 + f % MT * 16 + r, n = n0 + f / MT * 16 + q * 4;
     if (at >= mend || n >= p.N) continue;
+    if constexpr (TY == GT_FP8)
+      if (zero4(sum) != 0) sum = fp8_again(p, g, at, n, 0, p.K, sum);
     const int have = min(4, p.N - n);
     if (p.accum) {
 #pragma unroll

@@ -191,3 +191,59 @@ def test_capture_beside_a_living_graph_of_a_view():
         torch.cuda.synchronize()
         assert torch.equal(taken[0], want) and torch.equal(taken[2], want)
         assert torch.equal(taken[1], alive)
+
+
+def far_scales(sizes, k, n, meet):
+    """Operands with a block pair whose scales' product passes float32 while
+    the values' products do not: 0 everywhere, or 2^119 at one k. Also the
+    operands without that pair."""
+    a = randn(sum(sizes), k, seed=14, dtype=torch.bfloat16)
+    w = randn(len(sizes), n, k, seed=15, dtype=torch.bfloat16)
+    at = 128 if k > 256 else 0
+    a[:, at:at + 128], w[..., at:at + 128] = 0, 0
+    a0, w0 = a.clone(), w.clone()
+    a[:, at + 1], w[..., at + 2] = 2.0 ** 75, 2.0 ** 72
+    if meet:  # 1.75 * 2^-6 in both payloads
+        a[:, at + 5], w[..., at + 5] = 2.0 ** 61, 2.0 ** 58
+    return a, w, a0, w0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("meet", [False, True])
+@pytest.mark.parametrize("sizes,k,n", [
+    ([3], 384, 200), ([2, 3], 389, 200), ([20, 9], 384, 72),  # few rows
+    ([70], 4096, 200),                                        # split sums
+    ([70, 1, 60], 384, 136), ([70, 1, 60], 389, 136),
+    ([100, 100], 7, 40),
+    ([2000, 1, 2099], 320, 1032), ([1300, 1, 1299], 320, 4104)])
+def test_fp8_scales_beyond_float32(sizes, k, n, meet, device):
+    """Sums are taken again by values there, without the matrix unit: nothing
+    is cut off but in the other blocks of a split sum."""
+    a, w, a0, w0 = (t.to(device) for t in far_scales(sizes, k, n, meet))
+    off = offsets_of(sizes, device)
+    qa, qw = ma.quantize_fp8(a), ma.quantize_fp8(w, "tile")
+    want = plain_rows(values_of(qa), values_of(qw).transpose(1, 2), off)
+    cut = fp8_cut(ma.quantize_fp8(a0), ma.quantize_fp8(w0, "tile"), off)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = ma.fp8_matmul(qa, qw, off, dtype)
+        assert_near(y, *want, k, cut)
+    # what is not finite by its values stays so, and in its place
+    a[1, 0] = float("inf")
+    y = ma.fp8_matmul(a, qw, off, torch.float32)
+    assert torch.isnan(y[1]).all()
+    y[1] = 0
+    assert torch.isfinite(y).all()
+
+
+@pytest.mark.gpu
+def test_fp8_scales_beyond_float32_accumulate():
+    from matrel_amd.ops import blockops
+    a, w, _, _ = (t.cuda() for t in far_scales([90], 384, 72, False))
+    qa, sa = blockops.to_fp8(a, "row")
+    qb, sb = blockops.to_fp8(w[0], "tile")
+    acc = torch.full((90, 72), 3.0, device="cuda")
+    blockops.gemm_bt_fp8_acc(acc, qa, sa, qb, sb, beta0=True)
+    one = acc.clone()
+    assert torch.isfinite(one).all()
+    blockops.gemm_bt_fp8_acc(acc, qa, sa, qb, sb)
+    assert torch.equal(acc, 2 * one)
