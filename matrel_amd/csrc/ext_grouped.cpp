@@ -466,18 +466,28 @@ c10::optional<Tensor> given(const Tensor& offs) {
   return offs.defined() ? c10::optional<Tensor>(offs) : c10::nullopt;
 }
 
+// The one type of a gradient's product: the operands', to which a wider result's
+// gradient is rounded. It can lie outside of fp16's range (the products of
+// 1e5 and 1e-4 are not infinite): all is multiplied in float32 there.
+at::ScalarType product_type(const Tensor& grad, at::ScalarType ty) {
+  return ty == torch::kFloat16 && grad.scalar_type() != ty ? torch::kFloat32
+                                                           : ty;
+}
+
 Tensor grad_a(const Tensor& grad, const Tensor& b,
               const c10::optional<Tensor>& offs) {
-  return grouped_rows(grad, b.transpose(1, 2), offs, b.scalar_type());
+  return grouped_rows(grad, b.to(grad.scalar_type()).transpose(1, 2), offs,
+                      b.scalar_type());
 }
 
 // In the memory order of b, so that an optimizer walks both alike.
 Tensor grad_b(const Tensor& grad, const Tensor& a, const Tensor& b,
               const c10::optional<Tensor>& offs) {
+  const Tensor x = a.to(grad.scalar_type());
   if (b.stride(1) == 1 && b.size(1) > 1)
-    return grouped_weights(grad, a, offs, b.size(0), b.scalar_type())
+    return grouped_weights(grad, x, offs, b.size(0), b.scalar_type())
         .transpose(1, 2);
-  return grouped_weights(a, grad, offs, b.size(0), b.scalar_type());
+  return grouped_weights(x, grad, offs, b.size(0), b.scalar_type());
 }
 
 struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
@@ -492,9 +502,8 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     const at::NoGradGuard guard;
     const auto saved = ctx->get_saved_variables();
     const Tensor &a = saved[0], &b = saved[1], &offs = saved[2];
-    // the products need one type: a float32 result of 16-bit operands rounds
-    // its gradient to theirs
-    const Tensor grad = rows_contiguous(grads[0].to(a.scalar_type()));
+    const Tensor grad = rows_contiguous(
+        grads[0].to(product_type(grads[0], a.scalar_type())));
     Tensor da, db;
     if (ctx->needs_input_grad(0)) da = grad_a(grad, b, offs);
     if (ctx->needs_input_grad(1)) db = grad_b(grad, a, b, offs);
@@ -555,7 +564,8 @@ struct Fp8Matmul : torch::autograd::Function<Fp8Matmul> {
       // in the operands' own type: the sum runs over rows, along which
       // neither has its scales
       const auto shape = ctx->saved_data["w_shape"].toIntVector();
-      dw = grouped_weights(rows_contiguous(grad.to(a_type)), saved[0], offs,
+      const auto ty = product_type(grad, a_type);
+      dw = grouped_weights(rows_contiguous(grad.to(ty)), saved[0].to(ty), offs,
                            shape.size() == 2 ? 1 : shape[0],
                            (at::ScalarType)ctx->saved_data["w_type"].toInt())
                .reshape(shape);

@@ -24,7 +24,7 @@ import torch
 
 from .backend import require_ext, use_hip
 from .grouped import (check_capture, check_offsets, check_out_dtype,
-                      needs_grad, refuse_tangents, rows_product,
+                      needs_grad, product_type, refuse_tangents, rows_product,
                       weights_product)
 
 BLOCK = 128
@@ -194,7 +194,8 @@ class _CpuFp8Matmul(torch.autograd.Function):
             # in the operands' own type: the sum runs over rows, along which
             # neither has its scales
             groups = 1 if w.dim() == 2 else w.shape[0]
-            dw = weights_product(grad.to(a.dtype), a, offsets, groups,
+            ty = product_type(grad, a.dtype)
+            dw = weights_product(grad.to(ty), a.to(ty), offsets, groups,
                                  w.dtype).reshape(w.shape)
         return da, dw, None, None, None
 

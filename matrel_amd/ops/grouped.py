@@ -148,15 +148,27 @@ def grouped_matmul_grads(grad: torch.Tensor, a: torch.Tensor,
     if use_hip(a):
         refuse_tangents(grad, a, b)
     with torch.no_grad():
-        grad = grad.to(a.dtype)
+        grad = grad.to(product_type(grad, a.dtype))
         return (_grad_a(grad, b, offsets), _grad_b(grad, a, b, offsets))
 
 
+def product_type(grad: torch.Tensor, dtype: torch.dtype) -> torch.dtype:
+    """The one type of a gradient's product: the operands' dtype, to which a
+    wider result's gradient is rounded. It can lie outside of float16's range
+    (the products of 1e5 and 1e-4 are not infinite): all is multiplied in
+    float32 there."""
+    if dtype == torch.float16 and grad.dtype != dtype:
+        return torch.float32
+    return dtype
+
+
 def _grad_a(grad, b, offsets):
-    return rows_product(grad, b.transpose(1, 2), offsets, b.dtype)
+    return rows_product(grad, b.to(grad.dtype).transpose(1, 2), offsets,
+                        b.dtype)
 
 
 def _grad_b(grad, a, b, offsets):
+    a = a.to(grad.dtype)
     # in the memory order of b, so that an optimizer walks both alike
     if b.stride(1) == 1 and b.shape[1] > 1:
         return weights_product(grad, a, offsets, b.shape[0],
@@ -176,9 +188,7 @@ class _CpuGroupedMatmul(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         a, b, offsets = ctx.saved_tensors
-        # the products need one type: a float32 result of 16-bit operands
-        # rounds its gradient to theirs
-        grad = grad.to(a.dtype)
+        grad = grad.to(product_type(grad, a.dtype))
         da = _grad_a(grad, b, offsets) if ctx.needs_input_grad[0] else None
         db = _grad_b(grad, a, b, offsets) if ctx.needs_input_grad[1] else None
         return da, db, None, None

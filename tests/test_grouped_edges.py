@@ -247,3 +247,35 @@ def test_fp8_scales_beyond_float32_accumulate():
     assert torch.isfinite(one).all()
     blockops.gemm_bt_fp8_acc(acc, qa, sa, qb, sb)
     assert torch.equal(acc, 2 * one)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e5, 1e-9])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_wide_gradient_of_half_operands(layout, size, out, device):
+    """Gradients that float16 does not hold, of products that it does."""
+    hf = dict(dtype=torch.float16, device=device)
+    off = offsets_of([20, 0, 45], device)
+    unit = 1e-4 if size > 1 else 1e3
+    a = randn(65, 72, seed=16, scale=unit, **hf).requires_grad_()
+    w = randn(3, 40, 72, seed=17, scale=unit, **hf)
+    if layout == "kn":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    w.requires_grad_()
+    gy = randn(65, 40, seed=18, dtype=out, device=device, scale=size)
+    want_a = plain_rows(gy, w, off)
+    want_w = plain_weights(gy, a, off)
+    y = ma.grouped_matmul(a, w.transpose(1, 2), off, out)
+    da, dw = torch.autograd.grad(y, (a, w), gy)
+    assert da.dtype == dw.dtype == torch.float16
+    assert_near(da, *want_a, 40)
+    assert_near(dw, *want_w, 45)
+    da2, db2 = ma.grouped_matmul_grads(gy, a, w.transpose(1, 2), off)
+    assert torch.equal(da, da2) and torch.equal(dw, db2.transpose(1, 2))
+    y = ma.fp8_matmul(a, w, off, out)
+    da, dw = torch.autograd.grad(y, (a, w), gy)
+    assert_near(dw, *want_w, 45)
+    qg, qw = ma.quantize_fp8(gy), ma.quantize_fp8(w, "tile")
+    assert_near(da, *plain_rows(values_of(qg), values_of(qw), off), 40,
+                fp8_cut(qg, qw.transpose(), off))
