@@ -119,7 +119,8 @@ def _mxq_panel_scales(prec, n: int, bs: int, side: str,
     """Room for the scales of n bs x bs panels: packed e8m0 words for the MX
     tiers, float32 for fp8 (as _mxq_convert lays them out)."""
     if prec == "fp8":
-        return torch.empty(n, bs // 128, bs if side == "a" else bs // 128,
+        nb = (bs + 127) // 128
+        return torch.empty(n, nb, bs if side == "a" else nb,
                            dtype=torch.float32, device=device)
     return torch.empty(n, bs // 128, bs, dtype=torch.int32, device=device)
 
@@ -500,7 +501,8 @@ def summa_matmul(a: BlockMatrix, b: BlockMatrix, out: BlockMatrix) -> None:
     _prec = get_config().gemm_precision
     mxq = (_prec if _prec in _MXQ_PRECS else None) if (
         a.device.type == "cuda" and a.dtype == torch.bfloat16
-        and b.dtype == torch.bfloat16 and bs % 256 == 0) else None
+        and b.dtype == torch.bfloat16
+        and (bs % 256 == 0 or _prec == "fp8")) else None
     mx8 = mxq is not None
     pbytes = _mxq_pbytes(mxq, bs)  # payload bytes per row
 

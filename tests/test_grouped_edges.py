@@ -279,3 +279,56 @@ def test_wide_gradient_of_half_operands(layout, size, out, device):
     qg, qw = ma.quantize_fp8(gy), ma.quantize_fp8(w, "tile")
     assert_near(da, *plain_rows(values_of(qg), values_of(qw), off), 40,
                 fp8_cut(qg, qw.transpose(), off))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [200, 100, 72, 33])
+def test_engine_fp8_any_block_size(bs, monkeypatch):
+    """gemm_precision="fp8" multiplies 8-bit blocks of any size, local and by
+    SUMMA's panels (over RCCL with one rank)."""
+    import torch.distributed as dist
+    from matrel_amd.exec import runtime, summa
+    old = ma.get_config()
+    runtime.reset_runtime()
+    os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
+    os.environ.setdefault("MASTER_PORT", "29419")
+    dist.init_process_group("nccl", rank=0, world_size=1)
+    try:
+        s = ma.MatrelSession(ma.MatrelConfig(block_size=bs,
+                                             gemm_precision="fp8"))
+        m, k, n = 300, 250, 210
+        ta = randn(m, k, seed=19, dtype=torch.bfloat16, device="cuda")
+        tb = randn(k, n, seed=20, dtype=torch.bfloat16, device="cuda")
+        local = (s.from_dense(ta) @ s.from_dense(tb)).to_tensor()
+        a, b = s.from_dense(ta).plan.data, s.from_dense(tb).plan.data
+        out = ma.BlockMatrix(m, n, block_size=bs)
+        rt = runtime.get_runtime()
+        monkeypatch.setattr(type(rt), "is_distributed", True)
+        monkeypatch.setattr(type(rt), "row_group",
+                            lambda self, p: dist.group.WORLD)
+        monkeypatch.setattr(type(rt), "col_group",
+                            lambda self, q: dist.group.WORLD)
+        summa.summa_matmul(a, b, out)
+        panels = torch.cat([torch.cat([out.blocks[i, j] for j in
+                                       range(-(-n // bs))], 1)
+                            for i in range(-(-m // bs))])
+        exact = torch.zeros(m, n, dtype=torch.float64)
+        size, cut = torch.zeros_like(exact), torch.zeros_like(exact)
+        for p in range(0, k, bs):
+            qa = ma.quantize_fp8(ta[:, p:p + bs])
+            for j in range(0, n, bs):
+                qb = ma.quantize_fp8(tb[p:p + bs, j:j + bs].t()[None], "tile")
+                off = offsets_of([m], "cuda")
+                y, z = plain_rows(values_of(qa), values_of(qb).transpose(1, 2),
+                                  off)
+                exact[:, j:j + bs] += y
+                size[:, j:j + bs] += z
+                cut[:, j:j + bs] += fp8_cut(qa, qb, off)
+        for got in (local, panels):
+            assert got.shape == (m, n)
+            assert_near(got.to(torch.bfloat16), exact, size, k, cut)
+    finally:
+        monkeypatch.undo()
+        dist.destroy_process_group()
+        ma.set_config(old)
+        runtime.reset_runtime()
