@@ -297,13 +297,15 @@ struct Side {
         glds16(s + at[i], smem + lds + (i * NT + threadIdx.x) * 16);
       } else {
         // the same instruction by hand: the compiler, which knows these
-        // copies, waits for all of them before each transposing read
+        // copies, waits for all of them before each transposing read. What it
+        // writes to LDS is not declared for that reason: every read of it
+        // stands behind a wait for its count that clobbers memory
         const u32 to = __builtin_amdgcn_readfirstlane(
             (u32)(uintptr_t)(__attribute__((address_space(3))) char*)smem +
             lds + (i * NT + (threadIdx.x & ~63u)) * 16);
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\t"
                      "global_load_lds_dwordx4 %0, %1"
-                     :: "v"(at[i]), "s"(s), "s"(to));
+                     :: "v"(at[i]), "s"(s), "s"(to) : "m0");
       }
     }
   }
