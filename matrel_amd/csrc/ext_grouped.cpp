@@ -433,14 +433,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
     st = torch::empty({0}, of);
   }
   if (q.numel() == 0) return {q, s, qt, st};
-  TORCH_CHECK(rb * cb < (int64_t(1) << 24) && E < 65536,
-              "matrix is too large");
+  TORCH_CHECK(rb * cb < (int64_t(1) << 24), "matrix is too large");
   const int64_t ld = R > 1 ? x.stride(1) : 0, bld = E > 1 ? x.stride(0) : 0;
-  launch_fp8_quantize_tile(x.data_ptr(), ty, ld, bld, E, R, C, q.data_ptr(),
-                           both ? qt.data_ptr() : nullptr,
-                           s.data_ptr<float>(),
-                           both ? st.data_ptr<float>() : nullptr,
-                           stream_of(x));
+  const auto at = [](const Tensor& t, int64_t i) {
+    return (char*)t.data_ptr() + i * t.element_size();
+  };
+  for (int64_t e = 0; e < E; e += 65535)  // what a launch's grid holds
+    launch_fp8_quantize_tile(
+        at(x, e * bld), ty, ld, bld, std::min<int64_t>(E - e, 65535), R, C,
+        at(q, e * R * C), both ? at(qt, e * R * C) : nullptr,
+        (float*)at(s, e * rb * cb),
+        both ? (float*)at(st, e * rb * cb) : nullptr, stream_of(x));
   check_launch();
   return {q, s, qt, st};
 }

@@ -332,3 +332,39 @@ def test_engine_fp8_any_block_size(bs, monkeypatch):
         dist.destroy_process_group()
         ma.set_config(old)
         runtime.reset_runtime()
+
+
+@pytest.mark.gpu
+def test_quantize_many_matrices():
+    """More matrices than a launch's grid holds, and their product's step."""
+    x = randn(70000, 3, 5, seed=21, device="cuda")
+    r = ma.quantize_fp8(x, "tile")
+    want = ma.quantize_fp8(x.cpu(), "tile")
+    assert torch.equal(r.scale.cpu(), want.scale)
+    assert torch.equal(r.data.cpu().float(), want.data.float())
+    a = randn(70000, 5, seed=22, device="cuda").requires_grad_()
+    w = x.requires_grad_()
+    off = torch.arange(70001, device="cuda", dtype=torch.int32)
+    gy = randn(70000, 3, seed=23, device="cuda")
+    y = ma.fp8_matmul(a, w, off)
+    da, dw = torch.autograd.grad(y, (a, w), gy)
+    qa, qg = ma.quantize_fp8(a), ma.quantize_fp8(gy)
+    v = values_of(r)
+
+    def rows(p, m):  # one row a group
+        p = p[:, None, :]
+        return [torch.bmm(f(p), f(m).contiguous())[:, 0]
+                for f in (lambda t: t, torch.abs)]
+
+    # 5 and 3 products of one group of 8 neighbours
+    for got, q, m in ((y, qa, v.transpose(1, 2)), (da, qg, v)):
+        exact, size = rows(values_of(q), m)
+        top = (q.data.cpu().float().abs().amax(1).clamp(min=2.0 ** -6)
+               .double() * q.scale.cpu()[0].double())
+        wtop = (r.data.cpu().float().abs().amax((1, 2)).clamp(min=2.0 ** -6)
+                .double() * r.scale.cpu().reshape(-1).double())
+        cut = 7 * 2.0 ** -13 * (top * wtop)[:, None].expand_as(exact)
+        assert_near(got, exact, size, 8, cut)
+    p = gy.detach().cpu().double()[:, :, None] * a.detach().cpu().double()[
+        :, None, :]
+    assert_near(dw, p, p.abs(), 1)
