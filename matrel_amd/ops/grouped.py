@@ -86,7 +86,7 @@ def check_capture(*operands) -> None:
 
 
 def _cpu_rows(a, b, offsets, out_dtype):
-    out = torch.zeros(a.shape[0], b.shape[2])
+    out = a.new_zeros(a.shape[0], b.shape[2], dtype=torch.float32)
     v = [0, a.shape[0]] if offsets is None else offsets.tolist()
     for g, (lo, hi) in enumerate(zip(v, v[1:])):
         out[lo:hi] = a[lo:hi].float() @ b[g].float()
@@ -94,7 +94,7 @@ def _cpu_rows(a, b, offsets, out_dtype):
 
 
 def _cpu_weights(a, b, offsets, groups, out_dtype):
-    out = torch.zeros(groups, a.shape[1], b.shape[1])
+    out = a.new_zeros(groups, a.shape[1], b.shape[1], dtype=torch.float32)
     v = [0, a.shape[0]] if offsets is None else offsets.tolist()
     for g, (lo, hi) in enumerate(zip(v, v[1:])):
         out[g] = a[lo:hi].float().t() @ b[lo:hi].float()

@@ -368,3 +368,31 @@ def test_quantize_many_matrices():
     p = gy.detach().cpu().double()[:, :, None] * a.detach().cpu().double()[
         :, None, :]
     assert_near(dw, p, p.abs(), 1)
+
+
+def test_cpu_forms_under_other_defaults():
+    """Sums of CPU tensors are float32 ones on the CPU, whatever torch makes
+    tensors of by default."""
+    a, w = randn(40, 300, seed=24), randn(2, 24, 300, seed=25)
+    gy = randn(40, 24, seed=26)
+    off = offsets_of([15, 25], "cpu")
+
+    def step():
+        x, m = a.clone().requires_grad_(), w.clone().requires_grad_()
+        out = []
+        for y in (ma.grouped_matmul(x, m.transpose(1, 2), off),
+                  ma.fp8_matmul(x, m, off)):
+            out += [y.detach(), *torch.autograd.grad(y, (x, m), gy)]
+        return out
+
+    want = step()
+    for dtype in (torch.bfloat16, torch.float64):
+        torch.set_default_dtype(dtype)
+        try:
+            got = step()
+        finally:
+            torch.set_default_dtype(torch.float32)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    with torch.device("meta"):
+        got = step()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
