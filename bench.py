@@ -28,6 +28,9 @@ import torch.distributed as dist
 # N per GPU count: 1 -> config 2 (65k), 8 -> config 3 (256k)
 N_TABLE = {1: 65536, 2: 98304, 4: 163840, 8: 262144}
 CPU_N_TABLE = {1: 1024, 2: 2048, 4: 2048, 8: 4096}  # no-GPU smoke path
+# what each --precision multiplies in
+DTYPES = {"bf16": "bf16", "mx8": "fp8_mx", "mx6": "fp6_mx", "mx4": "fp4_mx",
+          "fp8": "fp8_block128"}
 
 
 def main():
@@ -39,9 +42,9 @@ def main():
                     help="override matrix side N")
     ap.add_argument("--block-size", type=int, default=0,
                     help="0 = auto (single block at 1 GPU, 16384 for SUMMA)")
-    ap.add_argument("--precision", choices=["bf16", "mx8", "mx6", "mx4", "fp8"],
-                    default="bf16",
-                    help="GEMM compute precision (mx8 = MX-scaled fp8; "
+    ap.add_argument("--precision", choices=list(DTYPES), default="bf16",
+                    help="GEMM compute precision (mx8 = MX-scaled fp8, fp8 = "
+                         "float32 scales per block of 128; "
                          "NOT the headline config - BASELINE is bf16)")
     args = ap.parse_args()
 
@@ -112,8 +115,7 @@ def main():
             "higher_is_better": True,
             "scaling": "weak",
             "vs_baseline": None,
-            "dtype": ({"mx8": "fp8_mx", "mx6": "fp6_mx", "mx4": "fp4_mx"}.get(args.precision, "bf16"))
-                     if has_gpu else "fp32",
+            "dtype": DTYPES[args.precision] if has_gpu else "fp32",
             "data": "synthetic",
             "config": {
                 "model": "NxN distributed dense matmul (BASELINE configs 2/3)",

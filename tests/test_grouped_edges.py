@@ -396,3 +396,13 @@ def test_cpu_forms_under_other_defaults():
     with torch.device("meta"):
         got = step()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_bench_names_the_precision():
+    import sys
+    sys.path.insert(0, os.path.dirname(os.path.dirname(
+        os.path.abspath(__file__))))
+    import bench
+    assert bench.DTYPES["bf16"] == "bf16"
+    assert len(set(bench.DTYPES.values())) == len(bench.DTYPES)
+    assert "fp8" in bench.DTYPES["fp8"]
