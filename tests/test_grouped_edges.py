@@ -406,3 +406,46 @@ def test_bench_names_the_precision():
     assert bench.DTYPES["bf16"] == "bf16"
     assert len(set(bench.DTYPES.values())) == len(bench.DTYPES)
     assert "fp8" in bench.DTYPES["fp8"]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("sizes,k,n", [
+    ([1], 8192, 1000), ([3], 8200, 200), ([3], 8195, 200),  # eight waves
+    ([3] * 20, 144, 6400), ([3] * 20, 145, 1400), ([20] * 20, 392, 1000),
+    ([20, 40], 4096, 300), ([70], 4096, 200), ([70], 4100, 333),
+    ([100, 100], 7, 140), ([33, 0, 129, 1, 62], 1000, 264),
+    ([33, 0, 129, 1, 62], 1001, 263), ([2000, 1, 2099], 392, 1032),
+    ([1300, 1, 1299], 392, 4104), ([2000, 1, 2099], 131, 4099)])
+def test_fp8_exact_sums(sizes, k, n, device):
+    """Payloads of -1, 0, 1 and scales of powers of two: every sum is a whole
+    number below 2^24 of its unit, no step rounds or cuts anything, and one
+    value, scale or tail off is a wrong result. 7 bits of 128 products, up to
+    7 of the scales and 7 of 65 K tiles make 21; the gradients' payloads, 448
+    = 7 * 2^6, make 24 with a factor that is a power of two."""
+    off = offsets_of(sizes, device)
+    g = torch.Generator().manual_seed(27)
+    t, e, kb, nb = sum(sizes), len(sizes), -(-k // 128), -(-n // 128)
+
+    def ints(*shape):
+        return torch.randint(-1, 2, shape, generator=g).float()
+
+    def powers(most, *shape):
+        return 2.0 ** torch.randint(0, most + 1, shape, generator=g)
+
+    f8 = torch.float8_e4m3fn
+    qa = ma.Fp8Blocks(ints(t, k).to(f8).to(device),
+                      powers(3, kb, t).to(device), "row")
+    qw = ma.Fp8Blocks(ints(e, n, k).to(f8).to(device),
+                      powers(4, e, kb, nb).to(device), "tile")
+    want = plain_rows(values_of(qa), values_of(qw).transpose(1, 2), off)
+    assert want[1].max() < 2.0 ** 24
+    y = ma.fp8_matmul(qa, qw, off, torch.float32)
+    assert torch.equal(y.cpu().double(), want[0])
+    # 448 is the largest value of a block: payloads of 448, scales as given
+    gy = ints(t, n) * 448 * powers(3, nb, t).repeat_interleave(
+        128, 0)[:n].t()
+    a = torch.zeros(t, k, device=device, requires_grad=True)
+    da, = torch.autograd.grad(ma.fp8_matmul(a, qw, off), a, gy.to(device))
+    want = plain_rows(gy, values_of(qw), off)
+    assert (want[1] / 448).max() < 2.0 ** 21
+    assert torch.equal(da.cpu().double(), want[0])
