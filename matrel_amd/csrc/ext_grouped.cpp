@@ -26,6 +26,7 @@ void launch_fp8_quantize_row(const void*, int, long, long, long, void*,
                              float*, hipStream_t);
 void launch_fp8_quantize_tile(const void*, int, long, long, long, long, long,
                               void*, void*, float*, float*, hipStream_t);
+void launch_fp8_turn(const void*, long, long, long, void*, hipStream_t);
 }
 
 namespace {
@@ -448,6 +449,25 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
   return {q, s, qt, st};
 }
 
+// e4m3 [E, R, C] -> [E, C, R]
+Tensor fp8_turn(Tensor q) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() &&
+              q.scalar_type() == torch::kFloat8_e4m3fn,
+              "needs contiguous e4m3 matrices");
+  const c10::hip::HIPGuard guard(q.device().index());
+  const int64_t E = q.size(0), R = q.size(1), C = q.size(2);
+  Tensor qt = torch::empty({E, C, R}, q.options());
+  if (q.numel() == 0) return qt;
+  TORCH_CHECK((R + 127) / 128 * ((C + 127) / 128) < (int64_t(1) << 24),
+              "matrix is too large");
+  for (int64_t e = 0; e < E; e += 65535)  // what a launch's grid holds
+    launch_fp8_turn((const char*)q.data_ptr() + e * R * C,
+                    std::min<int64_t>(E - e, 65535), R, C,
+                    (char*)qt.data_ptr() + e * R * C, stream_of(q));
+  check_launch();
+  return qt;
+}
+
 // ---- autograd --------------------------------------------------------------
 
 using torch::autograd::AutogradContext;
@@ -556,8 +576,8 @@ struct Fp8Matmul : torch::autograd::Function<Fp8Matmul> {
     if (ctx->needs_input_grad(0)) {
       Tensor bt = saved[1], bsc = saved[2];
       if (ctx->saved_data["frozen"].toBool()) {
-        bt = bt.view(torch::kUInt8).transpose(-1, -2).contiguous().view(
-            torch::kFloat8_e4m3fn);
+        bt = fp8_turn(bt.dim() == 3 ? bt : bt.unsqueeze(0));
+        if (bsc.dim() == 2) bsc = bsc.unsqueeze(0);
         bsc = bsc.transpose(-1, -2).contiguous();
       }
       da = grouped_rows_fp8(grad, c10::nullopt, bt, bsc, offs, a_type,
@@ -639,6 +659,7 @@ void bind_grouped(pybind11::module& m) {
         "e4m3 with a scale for each 128 of a row");
   m.def("fp8_quantize_tile", &fp8_quantize_tile,
         "e4m3 with a scale for each 128 x 128 tile");
+  m.def("fp8_turn", &fp8_turn, "e4m3 matrices transposed");
   m.def("grouped_matmul", &grouped_matmul, "differentiable grouped_rows");
   m.def("fp8_matmul", &fp8_matmul, "differentiable grouped_rows_fp8");
   m.def("capturing", &capturing,

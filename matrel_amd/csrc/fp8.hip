@@ -103,6 +103,25 @@ quantize_row_k(const void* __restrict__ x, long ld, long rows, long cols,
   if ((threadIdx.x & 15) == 0) scale[cb * rows + row] = t / 448.0f;
 }
 
+// A tile of 128 x 128 bytes in LDS, to its place in the transposed matrix: a
+// thread gathers 8 rows of one column, 16 lanes write its 128 rows.
+__device__ __forceinline__ void put_turned(const unsigned char (*turn)[132],
+                                           unsigned char* qt, long rows,
+                                           long cols, long rb, long cb) {
+  const long r8 = rb * 128 + (threadIdx.x & 15) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = (threadIdx.x >> 4) + i * 16;
+    u32 w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j >> 2] |= (u32)turn[(threadIdx.x & 15) * 8 + j][c] << (8 * (j & 3));
+    if (cb * 128 + c < cols && r8 < rows)
+      put8(qt + (cb * 128 + c) * rows + r8, make_uint2(w[0], w[1]),
+           (int)min(8L, rows - r8));
+  }
+}
+
 // A workgroup takes a tile of 128 x 128, 64 values a thread. With `qt` it also
 // writes the tile transposed (through LDS), for products along the other axis.
 template <int TY>
@@ -154,19 +173,41 @@ quantize_tile_k(const void* __restrict__ x, long ld, long batch_ld, long rows,
   }
   if (!qt) return;
   __syncthreads();
-  // a thread gathers 8 rows of one column: 16 lanes write its 128 rows
-  const long r8 = rb * 128 + (threadIdx.x & 15) * 8;
+  put_turned(turn, qt + e * rows * cols, rows, cols, rb, cb);
+}
+
+// e4m3 matrices transposed, where a program keeps blocks of one side only.
+// Bound by memory: 8 x 4096 x 2048 in 30 us, 4.4 TB/s read + written.
+__global__ void __launch_bounds__(256)
+turn_k(const unsigned char* __restrict__ q, long rows, long cols,
+       unsigned char* __restrict__ qt) {
+  __shared__ unsigned char turn[128][132];
+  const long nrb = (rows + 127) / 128, ncb = (cols + 127) / 128;
+  const u32 id = xcd_swizzle(blockIdx.x, (u32)(nrb * ncb));
+  const long cb = id % ncb, rb = id / ncb, e = blockIdx.y;
+  const long col = cb * 128 + (threadIdx.x & 15) * 8;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = (threadIdx.x >> 4) + i * 16;
-    u32 w[2] = {0, 0};
+    const int r = (threadIdx.x >> 4) + i * 16;
+    const long row = rb * 128 + r;
+    uint2 w = {0, 0};
+    if (row < rows && col < cols) {
+      const unsigned char* x = q + (e * rows + row) * cols + col;
+      if (col + 8 <= cols) {
+        __builtin_memcpy(&w, x, 8);
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      w[j >> 2] |= (u32)turn[(threadIdx.x & 15) * 8 + j][c] << (8 * (j & 3));
-    if (cb * 128 + c < cols && r8 < rows)
-      put8(qt + (e * cols + cb * 128 + c) * rows + r8, make_uint2(w[0], w[1]),
-           (int)min(8L, rows - r8));
+        for (int j = 0; j < 8; ++j)
+          if (col + j < cols)
+            (j < 4 ? w.x : w.y) |= (u32)x[j] << (8 * (j & 3));
+      }
+    }
+    u32* s = (u32*)&turn[r][(threadIdx.x & 15) * 8];
+    s[0] = w.x;
+    s[1] = w.y;
   }
+  __syncthreads();
+  put_turned(turn, qt + e * rows * cols, rows, cols, rb, cb);
 }
 
 extern "C" void launch_fp8_quantize_row(const void* x, int ty, long ld,
@@ -197,4 +238,12 @@ extern "C" void launch_fp8_quantize_tile(const void* x, int ty, long ld,
   else if (ty == GT_BF16) GO(GT_BF16);
   else GO(GT_F16);
 #undef GO
+}
+
+extern "C" void launch_fp8_turn(const void* q, long batch, long rows,
+                                long cols, void* qt, hipStream_t s) {
+  const dim3 grid((unsigned)(((cols + 127) / 128) * ((rows + 127) / 128)),
+                  (unsigned)batch);
+  hipLaunchKernelGGL(turn_k, grid, dim3(256), 0, s, (const unsigned char*)q,
+                     rows, cols, (unsigned char*)qt);
 }

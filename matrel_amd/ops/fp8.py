@@ -18,6 +18,7 @@ csrc/grouped_core.h), CPU tensors plain torch.
 from __future__ import annotations
 
 import dataclasses
+import math
 from typing import Optional, Union
 
 import torch
@@ -88,9 +89,15 @@ class Fp8Blocks:
         """The transposed matrices (kind "tile"): the same values, copied."""
         if self.kind != "tile":
             raise ValueError('only kind "tile" can be transposed')
-        d = self.data.view(torch.uint8).transpose(-1, -2).contiguous()
-        return Fp8Blocks(d.view(torch.float8_e4m3fn),
-                         self.scale.transpose(-1, -2).contiguous(), "tile")
+        d = self.data
+        if use_hip(d):
+            n, r, c = math.prod(d.shape[:-2]), d.shape[-2], d.shape[-1]
+            d = require_ext().fp8_turn(d.view(n, r, c)).view(
+                *d.shape[:-2], c, r)
+        else:
+            d = d.view(torch.uint8).transpose(-1, -2).contiguous().view(
+                torch.float8_e4m3fn)
+        return Fp8Blocks(d, self.scale.transpose(-1, -2).contiguous(), "tile")
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the blocks stand for."""

@@ -449,3 +449,20 @@ def test_fp8_exact_sums(sizes, k, n, device):
     want = plain_rows(gy, values_of(qw), off)
     assert (want[1] / 448).max() < 2.0 ** 21
     assert torch.equal(da.cpu().double(), want[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [
+    (1, 1), (1, 300), (300, 1), (128, 128), (130, 257), (3, 136, 264),
+    (2, 77, 111), (2, 3, 40, 9), (0, 4, 8), (2, 0, 8), (70000, 3, 5)])
+def test_transposed_blocks(shape, device):
+    """Bit for bit, every payload among them."""
+    g = torch.Generator().manual_seed(28)
+    d = torch.randint(0, 256, shape, generator=g, dtype=torch.uint8)
+    s = torch.rand(*shape[:-2], -(-shape[-1] // 128), -(-shape[-2] // 128),
+                   generator=g)
+    q = ma.Fp8Blocks(d.to(device).view(torch.float8_e4m3fn), s.to(device),
+                     "tile").transpose()
+    assert torch.equal(q.data.view(torch.uint8).cpu(), d.transpose(-1, -2))
+    assert torch.equal(q.scale.cpu(), s.transpose(-1, -2))
+    assert q.kind == "tile"
