@@ -52,8 +52,11 @@ void check_launch() {
   TORCH_CHECK(e == hipSuccess, "HIP error: ", hipGetErrorString(e));
 }
 
+// Kernels count in 32 bits, up to 16 parts of whole tiles or 32 K tiles of 128
+// bytes past the end.
 int dim32(int64_t n, const char* what) {
-  TORCH_CHECK(n >= 0 && n < (int64_t(1) << 31) - 512, what, " is too large");
+  TORCH_CHECK(n >= 0 && n < (int64_t(1) << 31) - (1 << 16), what,
+              " is too large");
   return (int)n;
 }
 

@@ -466,3 +466,17 @@ def test_transposed_blocks(shape, device):
     assert torch.equal(q.data.view(torch.uint8).cpu(), d.transpose(-1, -2))
     assert torch.equal(q.scale.cpu(), s.transpose(-1, -2))
     assert q.kind == "tile"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [(1 << 31) - (1 << 16), (1 << 31) - 600])
+def test_refuses_sizes_near_2_31(k):
+    """The last K tiles would be counted past 31 bits. (Nothing is allocated:
+    refused before the expanded operands are copied.)"""
+    one = torch.zeros(1, dtype=torch.bfloat16, device="cuda")
+    off = offsets_of([1], "cuda")
+    for a, b in ((one.expand(1, k), one.expand(1, k, 1)),
+                 (one.expand(k, 1), one.expand(1, 1, 1)),
+                 (one.expand(1, 1), one.expand(1, 1, k))):
+        with pytest.raises(RuntimeError, match="too large"):
+            ma.grouped_matmul(a, b, off)
