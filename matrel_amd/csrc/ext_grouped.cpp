@@ -608,12 +608,18 @@ Tensor fp8_matmul(Tensor a, c10::optional<Tensor> w, c10::optional<Tensor> q,
   return Fp8Matmul::apply(a, w, q, s, offs, (int64_t)out);
 }
 
-// Whether the current stream of t's device is being captured.
-bool capturing(const Tensor& t) {
+// Whether a stream is being captured. The default stream (id 0) never is, and
+// must not be asked while another thread captures.
+bool is_captured(const c10::hip::HIPStream& s) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  const hipError_t e = hipStreamIsCapturing(stream_of(t), &status);
+  if (s.id() == 0) return false;
+  const hipError_t e = hipStreamIsCapturing(s.stream(), &status);
   TORCH_CHECK(e == hipSuccess, "HIP error: ", hipGetErrorString(e));
   return status != hipStreamCaptureStatusNone;
+}
+
+bool capturing(const Tensor& t) {
+  return is_captured(c10::hip::getCurrentHIPStream(t.device().index()));
 }
 
 // Whether the backward pass behind t, a leaf or not, would run nodes on a
@@ -633,16 +639,9 @@ bool held_by_other_stream(const Tensor& t) {
     if (!node || !met.insert(node.get()).second) continue;
     if (const auto s = node->stream()) {
       // by id: the one is of device type "cuda", the other "hip"
-      if (s->id() != c10::hip::getCurrentHIPStream(s->device_index()).id()) {
-        // the default stream (0) is never captured
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (s->id() == 0 ||
-            hipStreamIsCapturing(
-                c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s)
-                    .stream(), &status) != hipSuccess ||
-            status == hipStreamCaptureStatusNone)
-          return true;
-      }
+      if (s->id() != c10::hip::getCurrentHIPStream(s->device_index()).id() &&
+          !is_captured(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s)))
+        return true;
     }
     for (const auto& edge : node->next_edges()) left.push_back(edge.function);
   }

@@ -252,7 +252,7 @@ def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
         check_offsets(offsets, bt.shape[0], a.shape[0], a.device)
     out_dtype = check_out_dtype(
         out_dtype, torch.bfloat16 if isinstance(a, Fp8Blocks) else a.dtype)
-    refuse_tangents(*(t for t in (a, bt) if isinstance(t, torch.Tensor)))
+    refuse_tangents(a, bt)
     if isinstance(a, Fp8Blocks):
         if isinstance(bt, torch.Tensor):
             if bt.requires_grad and torch.is_grad_enabled():

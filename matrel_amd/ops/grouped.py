@@ -58,14 +58,16 @@ def needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-def refuse_tangents(*tensors) -> None:
+def refuse_tangents(*operands) -> None:
     """Forward-mode tangents, which requires_grad does not show: the kernels
     carry none, and a result without one would count as constant."""
     if forward_ad._current_level < 0:
         return
-    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        raise NotImplementedError("grouped and 8-bit products have no "
-                                  "forward-mode derivative")
+    for t in operands:
+        if isinstance(t, torch.Tensor) \
+                and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("grouped and 8-bit products have no "
+                                      "forward-mode derivative")
 
 
 def check_capture(*operands) -> None:
