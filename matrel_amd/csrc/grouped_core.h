@@ -558,16 +558,19 @@ __device__ __forceinline__ f32x4 fp8_again(const GroupedArgs& p, int g,
   const unsigned char* a = (const unsigned char*)p.a + (long)row * p.lda;
   const unsigned char* b = (const unsigned char*)p.b + (long)g * p.gsb;
   f32x4 sum = {0, 0, 0, 0};
+  bool any = true;  // what has become infinite or NaN stays so
 #pragma unroll 1
-  for (int k = kbeg; k < kend; ++k) {
+  for (int k = kbeg; k < kend && any; ++k) {
     const float x = __builtin_amdgcn_cvt_f32_fp8(a[k], 0) *
                     xs[(long)(k / 128) * p.T];
+    any = false;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int n = min(col + q, p.N - 1);
       const float y = __builtin_amdgcn_cvt_f32_fp8(b[(long)n * p.ldb + k], 0) *
                       ys[(long)(k / 128) * nb];
       sum[q] = __builtin_fmaf(x, y, sum[q]);
+      any |= sum[q] - sum[q] == 0;
     }
   }
 #pragma unroll

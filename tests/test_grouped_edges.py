@@ -480,3 +480,20 @@ def test_refuses_sizes_near_2_31(k):
                  (one.expand(1, 1), one.expand(1, 1, k))):
         with pytest.raises(RuntimeError, match="too large"):
             ma.grouped_matmul(a, b, off)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("t", [5, 700])
+def test_fp8_results_beyond_float32(t, device):
+    """What is infinite by its values stays infinite, with its sign."""
+    k, n = 520, 300
+    a = torch.full((t, k), 2.0 ** 80, device=device)
+    w = torch.full((n, k), 2.0 ** 70, device=device)
+    w[1::2] *= -1
+    y = ma.fp8_matmul(a, w)
+    assert (y[:, ::2] == float("inf")).all()
+    assert (y[:, 1::2] == -float("inf")).all()
+    w[3, 400] = float("nan")
+    y = ma.fp8_matmul(a, w)  # its tile: columns 0 .. 127
+    assert torch.isnan(y[:, :128]).all()
+    assert torch.isinf(y[:, 128:]).all()
