@@ -218,7 +218,8 @@ def fp8_matmul(a: Union[torch.Tensor, Fp8Blocks],
                bt: Union[torch.Tensor, Fp8Blocks],
                offsets: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """a @ bt^T in 8 bits, sums in float32.
+    """a @ bt^T in 8 bits. The sums are float32 ones, but for what a GPU's
+    matrix unit cuts off the products of 8 neighbours (above).
 
     a [rows, k]: a tensor, quantized here by rows, or blocks of kind "row".
     bt [n, k], or [groups, n, k] with offsets (see grouped_matmul): a tensor,
