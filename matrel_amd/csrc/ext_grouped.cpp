@@ -75,6 +75,15 @@ bool near_rows(const Tensor& t, int64_t ld, int64_t len) {
          ld * t.element_size() < (1 << 23);
 }
 
+// t as the kernels can read it: what torch only marks as negated or as zeros
+// is written out, and a tensor without memory (a fake one) refused.
+Tensor readable(const Tensor& t) {
+  if (t.is_neg() || t._is_zerotensor()) return t.clone();
+  TORCH_CHECK(t.numel() == 0 || t.const_data_ptr() != nullptr,
+              "operands must have memory");
+  return t;
+}
+
 // t, or a copy whose last dimension is contiguous.
 Tensor rows_contiguous(const Tensor& t) {
   return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
@@ -86,7 +95,7 @@ void set_offsets(GroupedArgs& p, c10::optional<Tensor>& offs,
     TORCH_CHECK(groups == 1, "several groups need offsets");
     return;
   }
-  offs = offs->contiguous();
+  offs = readable(*offs).contiguous();
   TORCH_CHECK(offs->device() == a.device() && offs->dim() == 1 &&
                   offs->numel() == groups + 1 &&
                   (offs->scalar_type() == torch::kInt32 ||
@@ -227,6 +236,8 @@ Tensor grouped_rows(Tensor a, Tensor b, c10::optional<Tensor> offs,
   const int ty = type_of(a.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   set_offsets(p, offs, a, E);
+  a = readable(a);
+  b = readable(b);
   Tensor c = torch::empty({T, N}, a.options().dtype(out));
   if (c.numel() == 0) return c;
   if (E == 0 || K == 0) return c.zero_();
@@ -274,6 +285,8 @@ Tensor grouped_weights(Tensor a, Tensor b, c10::optional<Tensor> offs,
   const int ty = type_of(a.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   set_offsets(p, offs, a, E);
+  a = readable(a);
+  b = readable(b);
   Tensor c = torch::empty({E, M, N}, a.options().dtype(out));
   if (c.numel() == 0) return c;
   if (T == 0) return c.zero_();
@@ -333,11 +346,14 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
               bt.scalar_type() == torch::kFloat8_e4m3fn && bt.is_contiguous(),
               "operands do not match");
   const c10::hip::HIPGuard guard(a.device().index());
+  a = readable(a);
+  bt = readable(bt);
+  bsc = readable(bsc);
   const int64_t T = a.size(0), K = a.size(1), N = bt.size(1), E = bt.size(0);
   const int64_t kb = (K + 127) / 128, nb = (N + 127) / 128;
   Tensor asc;
   if (a_scales.has_value()) {
-    asc = *a_scales;
+    asc = readable(*a_scales);
     TORCH_CHECK(a.scalar_type() == torch::kFloat8_e4m3fn &&
                 a.is_contiguous(), "a with scales must be contiguous e4m3");
     TORCH_CHECK(asc.device() == a.device() &&
@@ -361,7 +377,8 @@ Tensor grouped_rows_fp8(Tensor a, c10::optional<Tensor> a_scales, Tensor bt,
   Tensor c;
   if (into.has_value()) {
     c = *into;
-    TORCH_CHECK(c.scalar_type() == torch::kFloat32 && c.is_contiguous() &&
+    TORCH_CHECK(!c.is_neg() && !c._is_zerotensor() &&
+                c.scalar_type() == torch::kFloat32 && c.is_contiguous() &&
                 c.device() == a.device() && c.dim() == 2 && c.size(0) == T &&
                 c.size(1) == N, "the result must be float32 [rows, columns]");
   } else {
@@ -397,7 +414,7 @@ std::tuple<Tensor, Tensor> fp8_quantize_row(Tensor x) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2);
   const c10::hip::HIPGuard guard(x.device().index());
   const int64_t R = x.size(0), C = x.size(1);
-  x = rows_contiguous(x);
+  x = rows_contiguous(readable(x));
   const int ty = type_of(x.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   Tensor q = torch::empty({R, C}, x.options().dtype(torch::kFloat8_e4m3fn));
@@ -421,7 +438,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_quantize_tile(Tensor x,
   TORCH_CHECK(x.is_cuda() && x.dim() == 3);
   const c10::hip::HIPGuard guard(x.device().index());
   const int64_t E = x.size(0), R = x.size(1), C = x.size(2);
-  x = rows_contiguous(x);
+  x = rows_contiguous(readable(x));
   const int ty = type_of(x.scalar_type());
   TORCH_CHECK(ty != GT_FP8);
   const int64_t rb = (R + 127) / 128, cb = (C + 127) / 128;
@@ -459,6 +476,7 @@ Tensor fp8_turn(Tensor q) {
               "needs contiguous e4m3 matrices");
   const c10::hip::HIPGuard guard(q.device().index());
   const int64_t E = q.size(0), R = q.size(1), C = q.size(2);
+  q = readable(q);
   Tensor qt = torch::empty({E, C, R}, q.options());
   if (q.numel() == 0) return qt;
   TORCH_CHECK((R + 127) / 128 * ((C + 127) / 128) < (int64_t(1) << 24),

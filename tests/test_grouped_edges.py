@@ -497,3 +497,36 @@ def test_fp8_results_beyond_float32(t, device):
     y = ma.fp8_matmul(a, w)  # its tile: columns 0 .. 127
     assert torch.isnan(y[:, :128]).all()
     assert torch.isinf(y[:, 128:]).all()
+
+
+@pytest.mark.gpu
+def test_operands_without_memory():
+    """What torch only marks as negated or zero is read as such; fake tensors
+    are refused before anything is launched."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    a = randn(9, 72, seed=31, device="cuda")
+    w = randn(2, 40, 72, seed=32, device="cuda")
+    off = offsets_of([4, 5], "cuda")
+    b = w.transpose(1, 2)
+    zero = torch._efficientzerotensor
+    for x, m in ((torch._neg_view(a), w), (a, torch._neg_view(w)),
+                 (zero(a.shape, device="cuda"), w),
+                 (a, zero(w.shape, device="cuda"))):
+        assert x.is_neg() or m.is_neg() or x._is_zerotensor() \
+            or m._is_zerotensor()
+        y, z = x.clone(), m.clone()
+        assert torch.equal(ma.grouped_matmul(x, m.transpose(1, 2), off),
+                           ma.grouped_matmul(y, z.transpose(1, 2), off))
+        assert torch.equal(ma.fp8_matmul(x, m, off), ma.fp8_matmul(y, z, off))
+    gy = zero((9, 40), device="cuda")
+    assert all((g == 0).all() for g in ma.grouped_matmul_grads(gy, a, b, off))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        x = torch.empty(9, 72, device="cuda")
+        for f in (lambda: ma.grouped_matmul(x, b, off),
+                  lambda: ma.fp8_matmul(x, w, off),
+                  lambda: ma.quantize_fp8(x),
+                  lambda: ma.quantize_fp8(x, "tile"),
+                  lambda: ma.grouped_matmul(a, b, torch.empty(
+                      3, dtype=torch.int32, device="cuda"))):
+            with pytest.raises(RuntimeError, match="must have memory"):
+                f()
