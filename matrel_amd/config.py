@@ -57,8 +57,8 @@ class MatrelConfig:
     # (MX-scaled fp4 e2m1, ~2x the fp8 rate at ~1-2 significant digits -
     # screening-pass precision) or "fp8" (e4m3 with a float32 scale for
     # each 128 of A's rows and each 128 x 128 tile of B; any block shape).
-    # All opt-in, for dense bfloat16 blocks on a GPU: other blocks multiply
-    # in their own type.
+    # All opt-in, for bfloat16 blocks on a GPU (sparse ones where they are
+    # multiplied densely); other blocks multiply in their own type.
     gemm_precision: str = "bf16"
 
     # --- sparsity ---
