@@ -510,9 +510,9 @@ c10::optional<Tensor> given(const Tensor& offs) {
   return offs.defined() ? c10::optional<Tensor>(offs) : c10::nullopt;
 }
 
-// The one type of a gradient's product: the operands', to which a wider result's
-// gradient is rounded. It can lie outside of fp16's range (the products of
-// 1e5 and 1e-4 are not infinite): all is multiplied in float32 there.
+// The one type of a gradient's product: the operands', to which the gradient of
+// a wider result is rounded. It can lie outside of fp16's range (the products
+// of 1e5 and 1e-4 are not infinite): all is multiplied in float32 there.
 at::ScalarType product_type(const Tensor& grad, at::ScalarType ty) {
   return ty == torch::kFloat16 && grad.scalar_type() != ty ? torch::kFloat32
                                                            : ty;
